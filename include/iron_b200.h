@@ -595,6 +595,69 @@ int iron_decode_step_bf16(const void* const* layer_ptrs, const void* maps, int L
                           int window, int* values, int* drawn, void* xa, void* xb, void* act,
                           void* logits, void* workspace, iron_stream_t stream);
 
+/* ------------------------------------------------------------------------------------
+ * A key/value cache in pages of 8-bit codes, for serving a batch of requests (the reference
+ * keeps one bf16 cache a sequence, iron/lm/blocks.py:627-733; none of these has a counterpart).
+ *   pool    (P, G, 2, page, D) e4m3: the keys [.., 0, ..] and the values [.., 1, ..] of one page
+ *           and KV head are one run of memory; D is 64 or 128, page 16, 32, 64, 128 or 256;
+ *   scales  (P, G, 2) f32, positive: a cached value is its code times its scale;
+ *   tables  (B, width) int32: request b's tokens i * page .. are in page tables[b][i];
+ *   lengths (B,) int32: tokens a request holds.
+ * Everything that changes from step to step is read on the device, so a captured call serves
+ * every step.  A page id outside 0 .. P - 1 is never followed: its tokens count as absent.
+ *
+ * iron_page_step: one step's bookkeeping.  new_tokens[b] >= 0 rows are appended to request b,
+ * a negative number ends it.  `pages` (P,) and `ring` = (head, count, -, -) are a ring of free
+ * page ids.  In request order, a request is served when its table is wide enough, its rows end
+ * within `rows`, and it needs no page or the pages needed up to and with it are not more than
+ * the ring holds; it takes its pages from the ring's head.  One that is not served keeps what
+ * it had and takes nothing.  Ended requests' pages go to the ring's tail in order, to be taken
+ * from the next step on.  Written: the new table entries, the ring's new tail, row_start (B + 1)
+ * (every request's rows, served or not), and for each of the `rows` rows slots (page id * page +
+ * offset; -1 past the last row and for a request that was not served) and positions;
+ * lengths_out (may be lengths) and ring_out = (head, count, requests not served, rows asked for;
+ * may be ring).  At most iron_page_step_max_requests() requests. */
+int iron_page_step_max_requests(void);
+int iron_page_step(int* tables, int width, const int* lengths, const int* new_tokens, int B,
+                   int* pages, int P, const int* ring, int page_size, int rows,
+                   int* lengths_out, int* ring_out, int* slots, int* positions, int* row_start,
+                   iron_stream_t stream);
+
+/* RoPE on the q and k of a step's rows (qkv (rows, (H + 2G) D), `pitch` elements between rows;
+ * angles (S, D) as iron_rope_bf16 takes them, row positions[r] clamped to the table), q to q_out
+ * (rows, H, D) in bf16, k (from the f32 rotation: one rounding) and v to slot slots[r] as codes.
+ * A page's scale is the smallest power of two, 2^-60 at least, under which its largest finite magnitude is
+ * at most 448; a page that goes on keeps the larger of its old and its new rows' scale, and codes
+ * already there are brought under it.  An infinity or NaN is stored as NaN and does not move the scale.
+ * Slots outside 0 .. P * page - 1 write nothing.  Rows that share a page must be consecutive,
+ * with consecutive slots, and no slot may come twice. */
+int iron_rope_kv_pages_e4m3(const void* qkv, long long pitch, const void* angles, void* q_out,
+                            void* pool, float* scales, int P, int page_size, const int* slots,
+                            const int* positions, int rows, int H, int G, int D, int S,
+                            iron_stream_t stream);
+
+/* One query a request, q (B, H, D), over its cache: out = softmax(scale * q K^T) V, f32 inside.
+ * window >= 0 keeps the keys within `window` positions of the last.  A request of length 0 gets
+ * zeros.  `workspace` (iron_mha_pages_workspace_bytes(D) bytes, 16-byte aligned) holds the call's
+ * partial results; it needs no clearing, and two calls that may overlap need one each. */
+long long iron_mha_pages_workspace_bytes(int D);
+int iron_mha_decode_pages_bf16(const void* q, const void* pool, const float* scales, int P,
+                               int page_size, const int* tables, int width, const int* lengths,
+                               int B, int H, int G, int D, int window, float scale,
+                               void* workspace, long long workspace_bytes, void* out,
+                               iron_stream_t stream);
+
+/* Ragged query rows, q (rows, H, D): request b's are row_start[b] .. row_start[b + 1] - 1 and sit
+ * at the last positions of its lengths[b] keys.  causal keeps the keys at or before a row's
+ * position (window >= 0: and within `window` of it); causal == 0 keeps all of a request's keys
+ * (states of another length) and takes no window.  Rows that see nothing are zeros; rows that
+ * belong to no request are left as they were. */
+int iron_mha_prefill_pages_bf16(const void* q, const void* pool, const float* scales, int P,
+                                int page_size, const int* tables, int width, const int* lengths,
+                                const int* row_start, int B, int rows, int H, int G, int D,
+                                int causal, int window, float scale, void* workspace,
+                                long long workspace_bytes, void* out, iron_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,49 @@
+// What the kernels of the paged 8-bit key/value cache share: the page sizes taken, the e4m3
+// conversions, and the power-of-two scale of a (page, KV head).
+#pragma once
+#include "common.cuh"
+
+namespace iron {
+
+constexpr int kMaxRequests = 8192;   // requests of one step (four words of shared memory each)
+
+// log2 of a page size the kernels take (16, 32, 64, 128 or 256 tokens), else -1.
+inline int log2_page(int page) {
+  for (int k = 4; k <= 8; ++k)
+    if (page == 1 << k) return k;
+  return -1;
+}
+
+// Two floats -> two e4m3 codes (to nearest even; NaN stays NaN), the first in the low byte.
+__device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Two e4m3 codes -> two halves (exact).
+__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t codes) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(codes));
+  return r;
+}
+__device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t codes) {
+  const uint32_t h = e4m3x2_to_half2(codes);
+  float2 f;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.f32.f16 %0, lo;\n\tcvt.f32.f16 %1, hi;\n\t}"
+      : "=f"(f.x), "=f"(f.y)
+      : "r"(h));
+  return f;
+}
+
+// 2^e, e the smallest whole number with amax <= 448 * 2^e, and 2^-60 at least (an all-zero page).
+// A float format rounds relative to the value, so a power of two costs no precision, and codes
+// that a later, larger scale moves are exact but for underflow.  448 = 1.75 * 2^8: with
+// amax = 1.f * 2^x, e = x - 8 where 1.f <= 1.75, else x - 7.
+__device__ __forceinline__ float pow2_scale(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  int e = (int)(u >> 23) - 127 - ((u & 0x7fffffu) <= 0x600000u ? 8 : 7);
+  e = max(e, -60);   // zero and subnormal magnitudes end here
+  return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+
+}  // namespace iron

@@ -568,6 +568,162 @@ def gemm_rows_qkv_rope(X, Wqkv, angles, q_out, k_cache, v_cache, positions, *, H
          H, G, D, k_cache.shape[1], _ptr(status), _stream())
 
 
+# ---- a key/value cache in pages of 8-bit codes ------------------------------------------------
+E4M3 = torch.float8_e4m3fn
+
+
+def _on_device(*ts) -> None:
+    """Every tensor is a contiguous one of the current CUDA device (launches go to its stream)."""
+    dev = torch.cuda.current_device() if torch.cuda.is_available() else None
+    for t in ts:
+        if not t.is_cuda:
+            raise RuntimeError("iron_b200 kernels take CUDA tensors only (no CPU fallback)")
+        if t.get_device() != dev:
+            raise ValueError(f"a tensor of cuda:{t.get_device()} in a call on cuda:{dev}")
+        if not t.is_contiguous():
+            raise ValueError("iron_b200 kernels take contiguous tensors")
+
+
+def _int32(**ts) -> None:
+    for name, t in ts.items():
+        if t.dtype != torch.int32:
+            raise TypeError(f"{name} is int32, not {t.dtype}")
+
+
+def _pool_sizes(pool, scales):
+    """(P, G, page, D) of a cache: ``pool`` (P, G, 2, page, D) e4m3, ``scales`` (P, G, 2) float32."""
+    if pool.dtype != E4M3 or scales.dtype != torch.float32:
+        raise TypeError(f"the pool is float8_e4m3fn and its scales float32, not {pool.dtype} and {scales.dtype}")
+    if pool.dim() != 5 or pool.shape[2] != 2 or scales.shape != pool.shape[:3]:
+        raise ValueError(f"pool {tuple(pool.shape)} and scales {tuple(scales.shape)} are not (P, G, 2, page, D) and (P, G, 2)")
+    return pool.shape[0], pool.shape[1], pool.shape[3], pool.shape[4]
+
+
+def page_step(tables, lengths, new_tokens, pages, ring, *, page_size, rows, lengths_out=None, ring_out=None,
+              slots=None, positions=None, row_start=None):
+    """One serving step's bookkeeping on the device: requests take pages, rows learn their slots.
+
+    ``tables`` (B, width), ``lengths`` and ``new_tokens`` (B,), ``pages`` (P,) and ``ring`` (4,) are
+    int32.  ``new_tokens[b]`` rows are appended to request ``b``; a negative number ends it and
+    gives its pages back.  ``tables`` and ``pages`` are updated in place; ``lengths_out`` and
+    ``ring_out`` may be ``lengths`` and ``ring``.  ``rows`` is how many rows the step's buffers hold.
+
+    Returns ``(slots, positions, row_start, lengths_out, ring_out)``; ``ring_out`` is (head, pages
+    free, requests not served, rows asked for).  A request that was not served keeps its length,
+    and its rows' slots are -1, as are those past the last row."""
+    if tables.dim() != 2 or lengths.dim() != 1 or new_tokens.shape != lengths.shape or tables.shape[0] != lengths.shape[0]:
+        raise ValueError(f"tables {tuple(tables.shape)}, lengths {tuple(lengths.shape)} and new_tokens "
+                         f"{tuple(new_tokens.shape)} are not (B, width), (B,) and (B,)")
+    if pages.dim() != 1 or ring.shape != (4,):
+        raise ValueError(f"pages {tuple(pages.shape)} and ring {tuple(ring.shape)} are not (P,) and (4,)")
+    B, width = tables.shape
+    if rows < 0:
+        raise ValueError(f"rows ({rows}) is negative")
+    device = tables.device
+    new = lambda n: torch.empty(n, dtype=torch.int32, device=device)  # noqa: E731
+    slots = new(rows) if slots is None else slots
+    positions = new(rows) if positions is None else positions
+    row_start = new(B + 1) if row_start is None else row_start
+    lengths_out = new(B) if lengths_out is None else lengths_out
+    ring_out = new(4) if ring_out is None else ring_out
+    if (slots.shape, positions.shape, row_start.shape) != ((rows,), (rows,), (B + 1,)) or \
+            lengths_out.shape != lengths.shape or ring_out.shape != ring.shape:
+        raise ValueError("outputs are slots (rows,), positions (rows,), row_start (B + 1,), lengths_out (B,), ring_out (4,)")
+    _int32(tables=tables, lengths=lengths, new_tokens=new_tokens, pages=pages, ring=ring, slots=slots,
+           positions=positions, row_start=row_start, lengths_out=lengths_out, ring_out=ring_out)
+    _on_device(tables, lengths, new_tokens, pages, ring, slots, positions, row_start, lengths_out, ring_out)
+    call("iron_page_step", tables.data_ptr(), width, lengths.data_ptr(), new_tokens.data_ptr(), B, pages.data_ptr(),
+         pages.shape[0], ring.data_ptr(), int(page_size), int(rows), lengths_out.data_ptr(), ring_out.data_ptr(),
+         slots.data_ptr(), positions.data_ptr(), row_start.data_ptr(), _stream())
+    return slots, positions, row_start, lengths_out, ring_out
+
+
+def rope_kv_pages(qkv, angles, q_out, pool, scales, slots, positions, *, H, G, D):
+    """RoPE on a step's q and k; q to ``q_out`` (rows, H, D), k and v into the paged cache's slots.
+
+    ``qkv`` (rows, (H + 2G) * D) bf16, its rows any pitch that is a multiple of 8 elements apart;
+    ``angles`` (S, D) bf16; ``slots`` and ``positions`` (rows,) int32 as ``page_step`` leaves them.
+    A page's scale is a power of two and only grows while the page fills."""
+    _bf16(qkv, angles, q_out)
+    P, PG, page, PD = _pool_sizes(pool, scales)
+    if (PG, PD) != (G, D):
+        raise ValueError(f"the pool holds {PG} heads of {PD}, not {G} of {D}")
+    rows = qkv.shape[0]
+    if qkv.dim() != 2 or qkv.shape[1] != (H + 2 * G) * D or qkv.stride(1) != 1:
+        raise ValueError(f"qkv {tuple(qkv.shape)} (strides {qkv.stride()}) is not rows of {(H + 2 * G) * D} adjacent elements")
+    if q_out.numel() != rows * H * D or slots.shape != (rows,) or positions.shape != (rows,):
+        raise ValueError(f"q_out {tuple(q_out.shape)}, slots {tuple(slots.shape)} and positions {tuple(positions.shape)} "
+                         f"are not for {rows} rows")
+    if angles.dim() != 2 or angles.shape[1] != D:
+        raise ValueError(f"angles {tuple(angles.shape)} are not (positions, {D})")
+    _int32(slots=slots, positions=positions)
+    _on_device(qkv[:1], angles, q_out, pool, scales, slots, positions)
+    call("iron_rope_kv_pages_e4m3", qkv.data_ptr(), qkv.stride(0) if rows > 1 else qkv.shape[1], angles.data_ptr(),
+         q_out.data_ptr(), pool.data_ptr(), scales.data_ptr(), P, page, slots.data_ptr(), positions.data_ptr(), rows,
+         H, G, D, angles.shape[0], _stream())
+    return q_out
+
+
+def pages_workspace(D: int, device=None) -> torch.Tensor:
+    """The partial results of one attention call over a paged cache; calls that may overlap need one each."""
+    return torch.empty(_lib.load().iron_mha_pages_workspace_bytes(D), dtype=torch.uint8, device=device or "cuda")
+
+
+def _pages_attention(Q, pool, scales, tables, lengths, out, workspace):
+    _bf16(Q, out)
+    P, G, page, D = _pool_sizes(pool, scales)
+    if Q.dim() != 3 or Q.shape[2] != D or Q.shape[1] % G:
+        raise ValueError(f"Q {tuple(Q.shape)} is not (rows, a multiple of {G} heads, {D})")
+    if tables.dim() != 2 or lengths.shape != tables.shape[:1]:
+        raise ValueError(f"tables {tuple(tables.shape)} and lengths {tuple(lengths.shape)} are not (B, width) and (B,)")
+    if out is None:
+        out = torch.empty_like(Q)
+    elif out.shape != Q.shape:
+        raise ValueError(f"out {tuple(out.shape)} is not {tuple(Q.shape)}")
+    if workspace is None:
+        workspace = pages_workspace(D, Q.device)
+    _int32(tables=tables, lengths=lengths)
+    _on_device(Q, out, pool, scales, tables, lengths, workspace)
+    return P, G, page, D, out, workspace
+
+
+def mha_decode_pages(Q, pool, scales, tables, lengths, out=None, *, window=None, scale=None, workspace=None):
+    """One query a request, ``Q`` (B, H, D), over the paged cache's first ``lengths[b]`` tokens.
+
+    ``window`` keeps the keys within that many positions of the last.  ``workspace``:
+    ``pages_workspace``'s buffer, allocated for the call when not given."""
+    if Q.shape[:1] != lengths.shape:
+        raise ValueError(f"Q {tuple(Q.shape)} is not one query for each of {tuple(lengths.shape)} requests")
+    P, G, page, D, out, workspace = _pages_attention(Q, pool, scales, tables, lengths, out, workspace)
+    call("iron_mha_decode_pages_bf16", Q.data_ptr(), pool.data_ptr(), scales.data_ptr(), P, page, tables.data_ptr(),
+         tables.shape[1], lengths.data_ptr(), Q.shape[0], Q.shape[1], G, D, -1 if window is None else int(window),
+         1.0 / math.sqrt(D) if scale is None else float(scale), workspace.data_ptr(), workspace.numel(),
+         out.data_ptr(), _stream())
+    return out
+
+
+def mha_prefill_pages(Q, pool, scales, tables, lengths, row_start, out=None, *, causal=True, window=None, scale=None,
+                      workspace=None):
+    """Ragged query rows over the paged cache: request ``b``'s are ``Q[row_start[b]:row_start[b + 1]]``,
+    at the last positions of its ``lengths[b]`` tokens.
+
+    ``causal=False`` lets every row see all of its request's tokens (and takes no ``window``).
+    Rows past ``row_start[B]`` are left as they were."""
+    B = lengths.shape[0]
+    if row_start.shape != (B + 1,):
+        raise ValueError(f"row_start {tuple(row_start.shape)} is not ({B + 1},)")
+    if window is not None and not causal:
+        raise ValueError("a window goes with the causal mask")
+    _int32(row_start=row_start)
+    P, G, page, D, out, workspace = _pages_attention(Q, pool, scales, tables, lengths, out, workspace)
+    _on_device(row_start)
+    call("iron_mha_prefill_pages_bf16", Q.data_ptr(), pool.data_ptr(), scales.data_ptr(), P, page, tables.data_ptr(),
+         tables.shape[1], lengths.data_ptr(), row_start.data_ptr(), B, Q.shape[0], Q.shape[1], G, D, int(bool(causal)),
+         -1 if window is None else int(window), 1.0 / math.sqrt(D) if scale is None else float(scale),
+         workspace.data_ptr(), workspace.numel(), out.data_ptr(), _stream())
+    return out
+
+
 def sample_k_max() -> int:
     """The largest top-k the device draws."""
     return _lib.load().iron_sample_k_max()

@@ -1,0 +1,509 @@
+"""The paged 8-bit cache on a B200: every operator against its plain form, and a run of them together."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from tests import pages_ref as R
+from tests.util import to_numpy
+
+pytestmark = pytest.mark.gpu
+
+BF16, F8, I32 = torch.bfloat16, torch.float8_e4m3fn, torch.int32
+
+
+def ints(x):
+    return torch.as_tensor(np.asarray(x), dtype=I32).cuda()
+
+
+# ---------------------------------------------------------------------------- page_step
+def step_inputs(B, width, page, seed, free, ended, new_hi, full=False):
+    rng = np.random.default_rng(seed)
+    lengths = rng.integers(0, width * page + 1, B) if full else rng.integers(0, max(1, width * page - new_hi), B)
+    new = np.where(rng.random(B) < ended, -1, rng.integers(0, new_hi + 1, B))
+    held = -(-lengths // page)
+    P = int(held.sum()) + free + 3
+    ids = rng.permutation(P)
+    tables = np.full((B, width), -1)
+    at = 0
+    for b in range(B):
+        tables[b, :held[b]] = ids[at:at + held[b]]
+        at += held[b]
+    head = int(rng.integers(P))
+    pages = np.full(P, -1)
+    pages[(head + np.arange(free)) % P] = ids[at:at + free]
+    return tables, lengths, new, pages, np.array([head, free, 0, 0])
+
+
+def check_step(got, tables, pages, want):
+    slots, positions, row_start, lengths, ring = (t.cpu().numpy() for t in got)
+    for name, x in dict(slots=slots, positions=positions, row_start=row_start, lengths=lengths, ring=ring,
+                        tables=tables.cpu().numpy(), pages=pages.cpu().numpy()).items():
+        assert np.array_equal(x, want[name]), name
+
+
+@pytest.mark.parametrize("B, width, page, free, ended, new_hi, rows", [
+    (1, 1, 16, 1, 0.0, 1, 1),
+    (3, 4, 16, 0, 0.3, 5, 20),               # nothing free
+    (64, 9, 64, 200, 0.1, 3, 128),
+    (65, 33, 16, 7, 0.2, 30, 2000),          # the ring runs out
+    (300, 17, 32, 900, 0.1, 90, 4000),       # the rows run out (and the cluster form)
+    (1025, 5, 128, 1500, 0.1, 2, 1500),      # more than one round of requests
+    (2500, 3, 256, 100, 0.5, 600, 100000),
+])
+@pytest.mark.parametrize("full", [False, True], ids=["room", "full tables"])
+def test_page_step(B, width, page, free, ended, new_hi, rows, full):
+    from iron_b200 import kernels as K
+
+    tables, lengths, new, pages, ring = step_inputs(B, width, page, B + page, free, ended, new_hi, full)
+    want = R.page_step(tables, lengths, new, pages, ring, page, rows)
+    t, l, n, p, r = map(ints, (tables, lengths, new, pages, ring))
+    got = K.page_step(t, l, n, p, r, page_size=page, rows=rows)
+    check_step(got, t, p, want)
+    assert np.array_equal(l.cpu().numpy(), lengths) and np.array_equal(r.cpu().numpy(), ring)
+    # in place
+    t, p = ints(tables), ints(pages)
+    got = K.page_step(t, l, n, p, r, page_size=page, rows=rows, lengths_out=l, ring_out=r)
+    assert got[3] is l and got[4] is r
+    check_step(got, t, p, want)
+
+
+def test_page_step_without_requests_or_rows():
+    from iron_b200 import kernels as K
+
+    pages, ring = ints(np.arange(5)), ints([3, 2, 9, 9])
+    slots, _, row_start, _, out = K.page_step(ints(np.zeros((0, 4))), ints([]), ints([]), pages, ring, page_size=16, rows=3)
+    assert slots.tolist() == [-1, -1, -1] and row_start.tolist() == [0] and out.tolist() == [3, 2, 0, 0]
+    # no room for rows: a request that brings none is served, one that brings some is not
+    t = ints(np.full((2, 2), -1))
+    _, _, row_start, lengths, out = K.page_step(t, ints([0, 0]), ints([0, 4]), pages, ring, page_size=16, rows=0)
+    assert lengths.tolist() == [0, 0] and out.tolist() == [3, 2, 1, 4] and row_start.tolist() == [0, 0, 4]
+
+
+def test_pages_are_never_held_twice():
+    """Many steps in place: every page is free once or held once, and the tables say what the plain loop says."""
+    from iron_b200 import kernels as K
+
+    rng = np.random.default_rng(3)
+    B, width, page, P, rows = 40, 12, 16, 150, 300
+    tables, lengths, pages, ring = np.full((B, width), -1), np.zeros(B, int), np.arange(P), np.array([0, P, 0, 0])
+    t, l, p, r = map(ints, (tables, lengths, pages, ring))
+    for _ in range(60):
+        new = np.where(rng.random(B) < 0.1, -1, rng.integers(0, 12, B))
+        want = R.page_step(tables, lengths, new, pages, ring, page, rows)
+        got = K.page_step(t, l, ints(new), p, r, page_size=page, rows=rows, lengths_out=l, ring_out=r)
+        check_step(got, t, p, want)
+        tables, lengths, pages, ring = want["tables"], want["lengths"], want["pages"], want["ring"]
+        held = [x for b in range(B) for x in tables[b, :-(-lengths[b] // page)]]
+        free = [pages[(ring[0] + i) % P] for i in range(ring[1])]
+        assert sorted(held + free) == list(range(P))
+
+
+def test_page_step_survives_a_ring_that_says_nonsense():
+    """Counts and ids outside their ranges are wrong answers at most: everything stays inside its buffer."""
+    from iron_b200 import kernels as K
+
+    t, l, n, p = ints(np.full((3, 4), 77)), ints([5, 1 << 30, -4]), ints([100, -1, 20]), ints([-9, 1 << 30, 3])
+    before = t.clone()
+    got = K.page_step(t, l, n, p, ints([-7, 99, 0, 0]), page_size=16, rows=40)
+    assert got[2].tolist() == [0, 100, 100, 120] and got[4][1].item() >= 0
+    assert t.shape == before.shape and torch.cuda.synchronize() is None
+
+
+# ---------------------------------------------------------------------------- rope_kv_pages
+def write_case(H, G, D, page, before, new, seed, wild=False):
+    """Requests with ``before`` tokens bring ``new`` rows; the pool holds the pages the step touches."""
+    rng = np.random.default_rng(seed)
+    first = [b // page for b in before]
+    count = [-(-(b + n) // page) - f for b, n, f in zip(before, new, first)]
+    P = sum(count) + 2
+    ids = rng.permutation(P)
+    slots, positions, at = [], [], 0
+    for b, n, f, c in zip(before, new, first, count):
+        t = np.arange(b, b + n)
+        slots += list(ids[at + t // page - f] * page + t % page)
+        positions += list(t)
+        at += c
+    rows = len(slots)
+    qkv = rng.standard_normal((rows, (H + 2 * G) * D)).astype(np.float32)
+    qkv *= np.exp2(rng.integers(-6, 7, (rows, 1)))          # scales that grow from step to step
+    if wild and rows:
+        flat = qkv.reshape(-1)
+        flat[rng.integers(0, flat.size, 40)] = rng.choice([np.inf, -np.inf, np.nan, 3e38, 1e-40, 0.0], 40)
+        qkv[rows // 2, H * D:] = 0
+    S = max(positions, default=0) + 3
+    a = np.arange(S)[:, None] * 10000.0 ** (-np.arange(0, D, 2) / D)
+    angles = np.stack((np.cos(a), np.sin(a)), -1).reshape(S, D)
+    qkv, angles = (torch.from_numpy(x.astype(np.float32)).to(BF16) for x in (qkv, angles))
+    pool, scales = R.cache(P, G, page, D, seed, device="cpu")
+    return qkv, angles, pool, scales, np.array(slots, int), np.array(positions, int)
+
+
+def check_write(q_out, pool, scales, want):
+    q, codes, sc = want
+    assert torch.equal(q_out.cpu().view(torch.int16), torch.from_numpy(q).to(BF16).view(torch.int16)) or np.array_equal(
+        q_out.cpu().float().numpy(), torch.from_numpy(q).to(BF16).float().numpy(), equal_nan=True)
+    assert np.array_equal(scales.cpu().double().numpy(), sc)
+    assert np.array_equal(pool.cpu().double().numpy(), codes, equal_nan=True)
+
+
+@pytest.mark.parametrize("H, G, D, page, before, new", [
+    (1, 1, 64, 16, [0], [1]),
+    (4, 2, 64, 16, [15, 0, 31, 7], [1, 1, 1, 1]),
+    (8, 8, 128, 16, [3], [50]),
+    (5, 1, 128, 32, [0, 31, 5, 100], [40, 2, 9, 8]),           # runs of eight and nine rows
+    (6, 3, 64, 64, [70, 1, 0], [200, 64, 63]),
+    (12, 4, 128, 128, [100, 127], [29, 130]),
+    (2, 2, 64, 256, [17], [600]),
+])
+@pytest.mark.parametrize("wild", [False, True], ids=["normal", "with infinities and NaN"])
+def test_rope_kv_pages(H, G, D, page, before, new, wild):
+    from iron_b200 import kernels as K
+
+    qkv, angles, pool, scales, slots, positions = write_case(H, G, D, page, before, new, page + H, wild)
+    with np.errstate(all="ignore"):
+        want = R.write(qkv.float().numpy(), angles.float().numpy(), pool.double().numpy(), scales.numpy(), slots, positions, H, G, D)
+    pool, scales = pool.cuda(), scales.cuda()
+    q = torch.full((len(slots), H, D), 7.0, dtype=BF16, device="cuda")
+    assert K.rope_kv_pages(qkv.cuda(), angles.cuda(), q, pool, scales, ints(slots), ints(positions), H=H, G=G, D=D) is q
+    check_write(q, pool, scales, want)
+    # the same step once more finds its own rows and scales there: nothing changes
+    K.rope_kv_pages(qkv.cuda(), angles.cuda(), q, pool, scales, ints(slots), ints(positions), H=H, G=G, D=D)
+    check_write(q, pool, scales, want)
+
+
+def test_rows_without_a_slot_and_positions_past_the_table():
+    from iron_b200 import kernels as K
+
+    H, G, D, page = 4, 2, 64, 16
+    qkv, angles, pool, scales, slots, positions = write_case(H, G, D, page, [14, 3, 0], [20, 5, 9], 5)
+    slots[21:25] = [-1, 1 << 30, len(pool) * page, -7]          # rows of the second request
+    slots[-3:] = -1
+    positions[-1] = 10 ** 6                                      # clamped to the last angle row
+    want = R.write(qkv.float().numpy(), angles.float().numpy(), pool.double().numpy(), scales.numpy(), slots, positions, H, G, D)
+    pool, scales = pool.cuda(), scales.cuda()
+    # rows farther apart than their width
+    wide = torch.zeros((len(slots), (H + 2 * G) * D + 24), dtype=BF16, device="cuda")
+    wide[:, :-24] = qkv.cuda()
+    q = torch.empty((len(slots), H, D), dtype=BF16, device="cuda")
+    K.rope_kv_pages(wide[:, :-24], angles.cuda(), q, pool, scales, ints(slots), ints(positions), H=H, G=G, D=D)
+    check_write(q, pool, scales, want)
+
+
+def test_a_page_filled_token_by_token_keeps_its_values():
+    """Forty steps of one token whose size grows: every stored value stays within half a step of
+    its last code, plus what each change of scale lost below the smallest code."""
+    from iron_b200 import kernels as K
+
+    G, D, page, n = 2, 64, 64, 40
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn((n, 4 * G, D), generator=g) * torch.exp2(torch.arange(n) / 4 - 6)[:, None, None]
+    qkv = x[:, : 3 * G].reshape(n, -1).to(BF16).cuda()
+    angles = torch.zeros((64, D), dtype=BF16, device="cuda")
+    angles[:, 0::2] = 1                                          # no rotation
+    pool, scales = torch.zeros((1, G, 2, page, D), dtype=F8, device="cuda"), torch.ones((1, G, 2), device="cuda")
+    q = torch.empty((1, G, D), dtype=BF16, device="cuda")
+    for t in range(n):
+        K.rope_kv_pages(qkv[t:t + 1], angles, q, pool, scales, ints([t]), ints([t]), H=G, G=G, D=D)
+    want = qkv.double().reshape(n, 3 * G, D)[:, G:].reshape(n, 2, G, D).permute(2, 1, 0, 3)   # (G, 2, n, D)
+    got = (pool.double() * scales.double()[..., None, None])[0, :, :, :n]
+    # a normal code is off by half a step (2^-4); the smallest code is 2^-9 of the scale, and the halves of it lost
+    # under every earlier scale (each at most half the next) sum to no more than one such step
+    bound = want.abs() * 2.0 ** -4 + scales.double()[0, :, :, None, None] * 2.0 ** -9
+    assert (got - want).abs().le(bound).all()
+
+
+# ---------------------------------------------------------------------------- attention
+def tolerance(want, size):
+    """Half a bf16 step of the output, a half's half step for each probability (2^-11 of sum p |v| / sum p) twice
+    over for the f32 exponentials, sums and scores, and the smallest bf16 numbers."""
+    return want.abs() * 2.0 ** -8 + size * 2.0 ** -10 + 1e-30
+
+
+def check_attention(out, want, size):
+    out = out.double()
+    assert torch.equal(torch.isnan(out), torch.isnan(want))
+    ok = torch.isnan(want) | ((out - want).abs() <= tolerance(want, size))
+    assert ok.all(), f"{int((~ok).sum())} of {ok.numel()} beyond the bound, worst {float((out - want).abs().nan_to_num().max()):.3g}"
+
+
+def queries(rows, H, D, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn((rows, H, D), generator=g, device="cuda") * torch.exp2(
+        torch.randint(-3, 3, (rows, H, 1), generator=g, device="cuda").float())).to(BF16)
+
+
+def poison(pool, scales, tables, lengths, page):
+    """NaN codes wherever no request has a token."""
+    used = torch.zeros(pool.shape[0], page, dtype=torch.bool)
+    for b, n in enumerate(lengths):
+        for t in range(0, n, page):
+            used[int(tables[b, t // page]), : min(page, n - t)] = True
+    pool.view(torch.uint8).masked_fill_(~used[:, None, None, :, None].cuda(), 0x7F)
+
+
+@pytest.mark.parametrize("H, G, D", [(4, 4, 64), (8, 1, 64), (6, 2, 128), (32, 8, 64), (9, 1, 128), (16, 1, 128), (40, 2, 64), (7, 7, 128)])
+@pytest.mark.parametrize("page, lengths", [
+    (16, [1]), (64, [0, 1, 15, 16, 17, 64, 65]), (32, [700, 33, 0, 129]), (128, [3001]), (256, [255, 256, 257, 5])])
+def test_decode(H, G, D, page, lengths):
+    from iron_b200 import kernels as K
+
+    tables, P = R.tables_for(lengths, page, H + page, width=14 if page == 256 else 0)
+    pool, scales = R.cache(P, G, page, D, H * D + page)
+    poison(pool, scales, tables, lengths, page)
+    q = queries(len(lengths), H, D, 5)
+    t, l = ints(tables), ints(lengths)
+    for window in (None, 0, 40):
+        out = K.mha_decode_pages(q, pool, scales, t, l, window=window)
+        want, size = R.attention(q, pool, scales, t, lengths, range(len(lengths) + 1), window=window)
+        check_attention(out, want, size)
+
+
+def test_decode_many_short_and_a_few_long():
+    """Segments of very different lengths over every CTA's share, and shares that cut them."""
+    from iron_b200 import kernels as K
+
+    lengths = [1, 20000, 5, 0, 333, 4097] + [17 * i % 500 for i in range(90)]
+    H, G, D, page = 12, 4, 128, 32
+    tables, P = R.tables_for(lengths, page, 1)
+    pool, scales = R.cache(P, G, page, D, 2)
+    q, t, l = queries(len(lengths), H, D, 3), ints(tables), ints(lengths)
+    workspace = K.pages_workspace(D).fill_(0xFF)             # a workspace needs no clearing
+    out = K.mha_decode_pages(q, pool, scales, t, l, scale=0.03, workspace=workspace)
+    check_attention(out, *R.attention(q, pool, scales, t, lengths, range(len(lengths) + 1), scale=0.03))
+    again = K.mha_decode_pages(q, pool, scales, t, l, scale=0.03, workspace=workspace)
+    assert torch.equal(out, again)                           # the order of the sums is fixed
+
+
+@pytest.mark.parametrize("H, G, D, page, lengths, new", [
+    (4, 4, 64, 16, [1], [1]),
+    (8, 2, 64, 64, [100, 7, 64, 0, 300], [5, 7, 1, 0, 130]),
+    (6, 2, 128, 32, [257, 128, 129, 1], [128, 128, 129, 1]),
+    (16, 1, 128, 128, [1500], [333]),
+    (5, 5, 64, 16, [40, 700], [0, 650]),
+    (24, 8, 128, 64, [513, 2, 77], [512, 2, 76]),
+    (12, 1, 64, 256, [300, 900], [300, 11]),
+    (3, 3, 128, 32, [1000], [1000]),
+])
+@pytest.mark.parametrize("mask", ["causal", "window 0", "window 50", "all"])
+def test_prefill(H, G, D, page, lengths, new, mask):
+    from iron_b200 import kernels as K
+
+    kw = dict(causal=mask != "all", window=int(mask.split()[1]) if " " in mask else None)
+    tables, P = R.tables_for(lengths, page, H + page)
+    pool, scales = R.cache(P, G, page, D, H * D + page)
+    poison(pool, scales, tables, lengths, page)
+    start = np.concatenate(([0], np.cumsum(new)))
+    q = queries(int(start[-1]) + 3, H, D, 5)
+    out = torch.full_like(q, 9.0)
+    t, l = ints(tables), ints(lengths)
+    assert K.mha_prefill_pages(q, pool, scales, t, l, ints(start), out, **kw) is out
+    want, size = R.attention(q, pool, scales, t, lengths, start, **kw)
+    n = int(start[-1])
+    check_attention(out[:n], want[:n], size[:n])
+    assert (out[n:] == 9).all()                              # rows of no request stay as they were
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_more_rows_than_keys_and_rows_that_see_nothing(D):
+    from iron_b200 import kernels as K
+
+    lengths, start, page = [3, 0, 40], [0, 10, 14, 60], 16
+    tables, P = R.tables_for(lengths, page, 1)
+    pool, scales = R.cache(P, 2, page, D, 3)
+    q, t = queries(60, 4, D, 1), ints(tables)
+    out = K.mha_prefill_pages(q, pool, scales, t, ints(lengths), ints(start))
+    check_attention(out, *R.attention(q, pool, scales, t, lengths, start))
+    assert (out[:7] == 0).all() and (out[10:14] == 0).all()
+    out = K.mha_prefill_pages(q, pool, scales, t, ints(lengths), ints(start), causal=False)
+    check_attention(out, *R.attention(q, pool, scales, t, lengths, start, causal=False))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_nan_reaches_only_the_rows_that_see_it(D):
+    """NaN keys and values of single tokens inside a chunk, where earlier rows share the tile."""
+    from iron_b200 import kernels as K
+
+    n, page, G, H = 300, 32, 2, 6
+    tables, P = R.tables_for([n], page, 1)
+    pool, scales = R.cache(P, G, page, D, 3)
+    raw = pool.view(torch.uint8)
+    for token, kind, d in ((150, 1, 5), (151, 1, 0), (260, 1, D - 1), (200, 0, 7), (299, 1, 33)):
+        raw[int(tables[0, token // page]), token % G, kind, token % page, d] = 0xFF if token % 2 else 0x7F
+    q, t, l = queries(n, H, D, 1), ints(tables), ints([n])
+    for kw in (dict(), dict(window=30)):
+        out = K.mha_prefill_pages(q, pool, scales, t, l, ints([0, n]), **kw)
+        want, size = R.attention(q, pool, scales, t, [n], [0, n], **kw)
+        assert torch.isnan(want).any() and not torch.isnan(want).all()
+        check_attention(out, want, size)
+    out = K.mha_decode_pages(q[-1:], pool, scales, t, l, window=30)
+    check_attention(out, *R.attention(q[-1:], pool, scales, t, [n], [0, 1], window=30))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_pages_outside_the_pool_count_as_absent(D):
+    from iron_b200 import kernels as K
+
+    lengths, new, page = [500, 70, 200], [200, 3, 1], 16
+    tables, P = R.tables_for(lengths, page, 1)
+    pool, scales = R.cache(P, 2, page, D, 3)
+    tables[0, 3], tables[0, 20], tables[1, :5], tables[2, 4] = -1, P, 1 << 30, -5
+    start, t, l = np.concatenate(([0], np.cumsum(new))), ints(tables), ints(lengths)
+    q = queries(sum(new), 4, D, 1)
+    out = K.mha_prefill_pages(q, pool, scales, t, l, ints(start))
+    check_attention(out, *R.attention(q, pool, scales, t, lengths, start))
+    out = K.mha_decode_pages(q[:3], pool, scales, t, l)
+    check_attention(out, *R.attention(q[:3], pool, scales, t, lengths, range(4)))
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+def test_scales_far_apart_and_scores_far_out(prompt):
+    """Page scales from 2^-30 to 2^20 that are no powers of two, queries of 2^-20 and 2^20, one key that takes all."""
+    from iron_b200 import kernels as K
+
+    n, page, G, H, D = 600, 16, 2, 4, 64
+    tables, P = R.tables_for([n, n], page, 1)
+    pool, scales = R.cache(P, G, page, D, 3)
+    g = torch.Generator(device="cuda").manual_seed(8)
+    scales[..., 1] *= torch.exp2(torch.rand(scales.shape[:2], generator=g, device="cuda") * 50 - 30)
+    scales[..., 0] *= 1.37
+    m = 200 if prompt else 1
+    q = queries(2 * m, H, D, 1)
+    q[:m] *= 2.0 ** -20
+    q[m:] *= 2.0 ** 5
+    start, t, l = [0, m, 2 * m], ints(tables), ints([n, n])
+    out = K.mha_prefill_pages(q, pool, scales, t, l, ints(start)) if prompt else K.mha_decode_pages(q, pool, scales, t, l)
+    want, size = R.attention(q, pool, scales, t, [n, n], start)
+    # scores of some thousands carry their f32 rounding (2^-24 each, of sums and of the product with log2 e) into the exponent
+    s = (q.double().abs().amax() * 448 * scales[..., 0].max().double() * math.sqrt(D))
+    size = size * (1 + float(s) * 2.0 ** -24 * 4 * 2 ** 10)
+    check_attention(out, want, size)
+
+
+def test_a_cache_past_four_gigabytes():
+    """Page offsets past 2^32 bytes: the pages in use are the pool's last."""
+    from iron_b200 import kernels as K
+
+    G, page, D, H = 8, 64, 128, 16
+    P = (5 << 30) // (G * 2 * page * D)
+    pool, scales = torch.zeros((P, G, 2, page, D), dtype=F8, device="cuda"), torch.ones((P, G, 2), device="cuda")
+    few, few_scales = R.cache(6, G, page, D, 1)
+    pool[-6:], scales[-6:] = few, few_scales
+    lengths, new = [200, 130], [90, 130]
+    local = np.array([[3, 0, 5, 1], [2, 4, 1, 0]])
+    q, l, start = queries(sum(new), H, D, 2), ints(lengths), [0, 90, 220]
+    want, size = R.attention(q, few, few_scales, ints(local), lengths, start)
+    check_attention(K.mha_prefill_pages(q, pool, scales, ints(local + P - 6), l, ints(start)), want, size)
+    want, size = R.attention(q[:2], few, few_scales, ints(local), lengths, [0, 1, 2])
+    check_attention(K.mha_decode_pages(q[:2], pool, scales, ints(local + P - 6), l), want, size)
+    # and the write: the last page, from its second half on
+    qkv, angles = queries(20, H + 2 * G, D, 4).reshape(20, -1), torch.ones((300, D), dtype=BF16, device="cuda")
+    slots, pos = np.arange(20) + (P - 1) * page + 40, np.arange(20)
+    ref = R.write(to_numpy(qkv.float()), np.ones((300, D), np.float32), few[-1:].double().cpu().numpy(),
+                  few_scales[-1:].cpu().numpy(), slots - (P - 1) * page, pos, H, G, D)
+    out = torch.empty((20, H, D), dtype=BF16, device="cuda")
+    K.rope_kv_pages(qkv, angles, out, pool, scales, ints(slots), ints(pos), H=H, G=G, D=D)
+    check_write(out, pool[-1:], scales[-1:], ref)
+    assert (pool[:1].view(torch.uint8) == 0).all()
+
+
+# ---------------------------------------------------------------------------- together
+def test_a_serving_run():
+    """Requests come, grow and end over many captured steps; each step's attention is held to the plain
+    form on the cache as it lies, and the cache to the rows that were written."""
+    from iron_b200 import kernels as K
+
+    rng = np.random.default_rng(11)
+    B, width, page, P, rows, H, G, D = 6, 10, 16, 40, 96, 8, 2, 64
+    tables, lengths, new = ints(np.full((B, width), -1)), ints(np.zeros(B)), ints(np.zeros(B))
+    pages, ring = ints(np.arange(P)), ints([0, P, 0, 0])
+    pool, scales = torch.zeros((P, G, 2, page, D), dtype=F8, device="cuda"), torch.ones((P, G, 2), device="cuda")
+    a = np.arange(width * page)[:, None] * 10000.0 ** (-np.arange(0, D, 2) / D)
+    angles = torch.from_numpy(np.stack((np.cos(a), np.sin(a)), -1).reshape(-1, D)).to(BF16).cuda()
+    qkv = torch.zeros((rows, (H + 2 * G) * D), dtype=BF16, device="cuda")
+    slots, positions, row_start = ints(np.zeros(rows)), ints(np.zeros(rows)), ints(np.zeros(B + 1))
+    q, out = torch.zeros((rows, H, D), dtype=BF16, device="cuda"), torch.zeros((rows, H, D), dtype=BF16, device="cuda")
+
+    def step():
+        K.page_step(tables, lengths, new, pages, ring, page_size=page, rows=rows, lengths_out=lengths, ring_out=ring,
+                    slots=slots, positions=positions, row_start=row_start)
+        K.rope_kv_pages(qkv, angles, q, pool, scales, slots, positions, H=H, G=G, D=D)
+        K.mha_prefill_pages(q, pool, scales, tables, lengths, row_start, out)
+
+    step()                                                   # nobody brings anything
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    history = [np.zeros((0, 2 * G, D)) for _ in range(B)]
+    for _ in range(40):
+        n = np.where(rng.random(B) < 0.12, -1, np.where(rng.random(B) < 0.3, rng.integers(0, 40, B), 1))
+        new.copy_(ints(n))
+        qkv.copy_(torch.from_numpy(rng.standard_normal(qkv.shape)).to(BF16))
+        was = lengths.cpu().numpy()
+        graph.replay()
+        torch.cuda.synchronize()
+        # a refused request's rows may be past the buffer: what there is of them is computed on what it had
+        now, start, x = lengths.cpu().numpy(), np.minimum(row_start.cpu().numpy(), rows), qkv.cpu().float().numpy().reshape(rows, -1, D)
+        for b in range(B):
+            if n[b] < 0:
+                assert now[b] == 0
+                history[b] = history[b][:0]
+            elif now[b] == was[b] + n[b]:
+                cs = angles.cpu().float().numpy()
+                fresh = [np.concatenate((R.rotate(x[start[b] + i], cs[was[b] + i])[H:H + G], x[start[b] + i, H + G:]))
+                         for i in range(n[b])]
+                history[b] = np.concatenate([history[b]] + [f[None] for f in fresh])
+            else:
+                assert now[b] == was[b]                      # refused: its rows went nowhere
+        served = int(start[-1])
+        want, size = R.attention(q, pool, scales, tables, now, start)
+        check_attention(out[:served], want[:served], size[:served])
+        for b in np.nonzero(now)[0]:
+            ids = tables[b, : -(-now[b] // page)].long()
+            got = (pool[ids].double() * scales[ids].double()[..., None, None]).permute(0, 3, 2, 1, 4).reshape(-1, 2 * G, D)
+            err = np.abs(got[: now[b]].cpu().numpy() - history[b])
+            sc = scales[ids].double().permute(0, 2, 1).reshape(-1, 1, 2 * G, 1).repeat(1, page, 1, 1).reshape(-1, 2 * G, 1)
+            # half a step of each of at most four scales a page goes through here (normal codes move exactly)
+            assert (err <= np.abs(history[b]) * 2.0 ** -4 + 2.0 ** -9 * sc[: now[b]].cpu().numpy()).all()
+
+
+def test_two_streams_and_two_graphs():
+    """Calls without a workspace of the caller's own may overlap: each has one, captured ones too."""
+    from iron_b200 import kernels as K
+
+    lengths, H, G, D, page = [9000, 37, 2500, 1], 8, 2, 128, 32
+    tables, P = R.tables_for(lengths, page, 1)
+    pool, scales = R.cache(P, G, page, D, 2)
+    t, l = ints(tables), ints(lengths)
+    qs = [queries(4, H, D, i) for i in range(4)]
+    want = [R.attention(q, pool, scales, t, lengths, range(5)) for q in qs]
+    K.mha_decode_pages(qs[0], pool, scales, t, l)
+    torch.cuda.synchronize()
+    streams, graphs, outs = [torch.cuda.Stream() for _ in range(4)], [], [torch.empty_like(q) for q in qs]
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            K.mha_decode_pages(qs[i], pool, scales, t, l, outs[i])
+    for _ in range(20):
+        for i in range(4):
+            with torch.cuda.stream(streams[i]):
+                if i < 2:
+                    graphs[i].replay()
+                else:
+                    K.mha_decode_pages(qs[i], pool, scales, t, l, outs[i])
+    torch.cuda.synchronize()
+    for out, w in zip(outs, want):
+        check_attention(out, *w)
+
+
+def test_a_tensor_of_another_kind_of_memory_is_refused():
+    from iron_b200 import kernels as K
+
+    pool, scales = R.cache(4, 1, 16, 64, 1)
+    q, t, l = queries(1, 1, 64, 1), ints([[0, 1]]), ints([20])
+    with pytest.raises(RuntimeError):
+        K.mha_decode_pages(q, pool, scales, t.cpu(), l)
+    with pytest.raises(ValueError):
+        K.mha_decode_pages(q, pool[:, :, :, ::2], scales, t, l)
