@@ -639,13 +639,14 @@ int iron_rope_kv_pages_e4m3(const void* qkv, long long pitch, const void* angles
 /* One query a request, q (B, H, D), over its cache: out = softmax(scale * q K^T) V, f32 inside.
  * window >= 0 keeps the keys within `window` positions of the last.  A request of length 0 gets
  * zeros.  `workspace` (iron_mha_pages_workspace_bytes(D) bytes, 16-byte aligned) holds the call's
- * partial results; it needs no clearing, and two calls that may overlap need one each. */
+ * partial results; it needs no clearing, and two calls that may overlap need one each.  `status`
+ * (may be NULL) receives IRON_ERR_TIMEOUT when a bounded wait of the pipeline gives up. */
 long long iron_mha_pages_workspace_bytes(int D);
 int iron_mha_decode_pages_bf16(const void* q, const void* pool, const float* scales, int P,
                                int page_size, const int* tables, int width, const int* lengths,
                                int B, int H, int G, int D, int window, float scale,
                                void* workspace, long long workspace_bytes, void* out,
-                               iron_stream_t stream);
+                               int* status, iron_stream_t stream);
 
 /* Ragged query rows, q (rows, H, D): request b's are row_start[b] .. row_start[b + 1] - 1 and sit
  * at the last positions of its lengths[b] keys.  causal keeps the keys at or before a row's
@@ -656,7 +657,8 @@ int iron_mha_prefill_pages_bf16(const void* q, const void* pool, const float* sc
                                 int page_size, const int* tables, int width, const int* lengths,
                                 const int* row_start, int B, int rows, int H, int G, int D,
                                 int causal, int window, float scale, void* workspace,
-                                long long workspace_bytes, void* out, iron_stream_t stream);
+                                long long workspace_bytes, void* out, int* status,
+                                iron_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -112,11 +112,11 @@ SIGNATURES: dict[str, tuple] = {
     "iron_mha_pages_workspace_bytes": (_L, [_I]),
     "iron_mha_decode_pages_bf16": (
         _I,
-        [_P, _P, _P, _I, _I, _P, _I, _P, _I, _I, _I, _I, _I, _F, _P, _L, _P, _P],
+        [_P, _P, _P, _I, _I, _P, _I, _P, _I, _I, _I, _I, _I, _F, _P, _L, _P, _P, _P],
     ),
     "iron_mha_prefill_pages_bf16": (
         _I,
-        [_P, _P, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P, _P],
+        [_P, _P, _P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P, _P, _P],
     ),
     "iron_mha_prefill_status_word": (None, [_P]),
     "iron_mha_prefill_bf16": (

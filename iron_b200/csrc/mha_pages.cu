@@ -1,25 +1,28 @@
 // Attention over a key/value cache that lies in pages of e4m3 codes, on warp MMAs: one query a
 // sequence (a decode step), or the few rows a sequence brings (a draft to verify, a short chunk).
 //
-// Bound by the cache's bytes, so the kernel is built around reading them once, in order, with
-// no staging: a warp's loads ARE the operand fragments.  Scores are computed transposed,
-// S^T = K Q^T (16 tokens x 8 query columns an MMA), and so is the output, O^T += V^T P^T, so a
-// group of up to eight query heads fills the MMA's narrow side and the codes its wide one:
+// Bound by the cache's bytes, so the kernel is built around keeping them coming: every warp has
+// a ring of its own in shared memory that TMA fills (16 tokens of one page and head a box, the
+// rows swizzled so that the fragment reads below meet no bank conflict), and no other warp to
+// wait for until its run of tokens ends.  Scores are computed transposed, S^T = K Q^T (16 tokens x
+// 8 query columns an MMA), and so is the output, O^T += V^T P^T, so a group of up to eight query
+// heads fills the MMA's narrow side and the codes its wide one:
 //   K fragment   lane (g, t) wants tokens g and g + 8, two adjacent elements a register.  Which
 //                elements make up "k" is free as long as Q agrees: lane t takes a run of D / 4
 //                consecutive codes of its tokens.
 //   V fragment   lane (g, t) wants tokens 2t, 2t + 1, 2t + 8, 2t + 9 of "rows" d; it takes the
 //                run of D / 8 codes at g * D / 8, and a byte permute pairs two tokens' codes.
 //   P            the score fragment holds tokens by rows; movmatrix turns it into the B operand.
-// Codes become halves exactly (one conversion a pair).  Q goes to halves too: each row times a
-// power of two that puts its largest element in [2^14, 2^15), so that elements down to 2^-31 of it
-// keep all their bits.  Scales join outside the products: a page's key scale multiplies its
-// scores, and the logarithm of its value scale is added to them, so that what is exponentiated
-// is a token's weight on the output, p * scale, under a running maximum of that weight (a maximum of p
-// alone would let a heavy page with small p push the others below half's range); the softmax's
-// denominator takes the weights over the scale again.  Weights are rounded to half (2^-11), held times
-// 2^10, so those down to 2^-24 of the largest keep full precision; scores, maxima, sums and
-// outputs are f32.
+// Codes become halves exactly (one conversion a pair; the e4m3 form of the MMA, with Q as two
+// codes an element, issued more instructions, not fewer: 398 a unit against 335).  Q goes to
+// halves too: each row times a power of two that puts its largest element in [2^14, 2^15), so that
+// elements down to 2^-31 of it keep all their bits.
+// Scales join outside the products: a page's key scale multiplies its scores, and the logarithm of
+// its value scale is added to them, so that what is exponentiated is a token's weight on the
+// output, p * scale, under a running maximum of that weight (a maximum of p alone would let a
+// heavy page with small p push the others below half's range); the softmax's denominator takes the
+// weights over the scale again.  Weights are rounded to half (2^-11), held times 2^10, so
+// those down to 2^-24 of the largest keep full precision; scores, maxima, sums and outputs are f32.
 //
 // Work is dealt out by the unit of 16 tokens: the units of all (sequence, KV head, column block)
 // segments, end to end, are cut into equal runs, one a CTA, so ragged lengths leave no CTA idle.
@@ -28,6 +31,7 @@
 #include "common.cuh"
 #include "mma.cuh"
 #include "pages.cuh"
+#include "tc.cuh"
 
 namespace iron {
 
@@ -36,7 +40,14 @@ constexpr int kPgThreads = kPgWarps * 32;
 constexpr int kPgCtasPerSm = 3;
 constexpr int kPgCtas = kSMs * kPgCtasPerSm;
 constexpr int kPgUnit = 16;                 // tokens
+constexpr int kPgStages = 2;                // of a warp's ring; a stage holds kGroup units
+constexpr int kPgSegCost = 16;              // units a segment costs beside its own (queries, merge)
 constexpr float kPgLift = 10.f;             // log2 of what probabilities are held times
+
+// A segment that several CTAs share, as the CTA that begins it leaves it for the fold.
+struct PagesRecord {
+  int pieces, row0, head0, col0, cols, pad[3];
+};
 
 struct PagesParams {
   const __nv_bfloat16* q;
@@ -47,14 +58,17 @@ struct PagesParams {
   const int* row_start;     // nullptr: one query a sequence
   __nv_bfloat16* out;
   float* partial;
-  int B, H, G, P, width, log_page, causal, window, rows, ctas;
+  PagesRecord* records;
+  int B, H, G, hg, P, width, log_page, causal, window, rows, ctas;   // hg = H / G
   float scale_log2;
+  int* status;
 };
 
 // A sequence as the kernels see it: its keys, its query rows, and the units a segment spans.
 struct PagesSeq {
   int len, row0, n, unit0;      // keys, first row, rows, first unit any row may see
-  int segs, units;              // segments (KV heads x column blocks) and units each
+  int blocks;                   // column blocks: G times as many segments
+  int units;                    // units of a segment
 };
 
 template <int COLS>
@@ -69,24 +83,39 @@ __device__ __forceinline__ PagesSeq pages_seq(const PagesParams& p, int b) {
   }
   const int first = p.window >= 0 ? max(0, s.len - s.n - p.window) : 0;
   s.unit0 = first / kPgUnit;
-  const int hg = p.H / p.G;
-  s.segs = p.G * (int)(((long long)s.n * hg + COLS - 1) / COLS);
+  s.blocks = (s.n * p.hg + COLS - 1) / COLS;
   // an empty segment still has a unit: somebody must write its zeros
   s.units = max(1, (s.len + kPgUnit - 1) / kPgUnit - s.unit0);
   return s;
 }
 
-// floats of one partial: COLS x D outputs, then COLS maxima and COLS sums
 template <int D, int NT>
 struct PgCfg {
   static constexpr int kCols = NT * 8;
-  static constexpr int kPartial = kCols * D + 2 * kCols;
+  static constexpr int kPartial = kCols * D + 2 * kCols;   // floats of a partial: outputs, maxima, sums
+  static constexpr int kGroup = D == 128 ? 2 : 4;          // units a warp takes at a time
+  static constexpr int kHalf = kPgUnit * D;                // bytes of a unit's keys, and of its values
+  static constexpr int kStage = kGroup * 2 * kHalf;        // 8 KB
+  static constexpr int kParts = NT * D <= 64 ? 1 : NT * D / 64;   // steps (of 8 KB) the warps' outputs meet in
+  static constexpr int kRing = 0;
+  static constexpr int kMerge = kPgWarps * kPgStages * kStage;
+  static constexpr int kBars = kMerge + kPgWarps * kCols * (D / kParts) * 4;
+  static constexpr int kSmem = kBars + 128 + 1024;
 };
 
-// units per CTA: an equal share, and two a warp at least
+// a / b for a >= 0, b > 0: the 64-bit division is a long routine, and seldom needed
+__device__ __forceinline__ long long div_ll(long long a, int b) {
+  return a >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
+// what a sequence's segments cost in units
+__device__ __forceinline__ long long pages_cost(const PagesParams& p, const PagesSeq& s) {
+  return (long long)p.G * s.blocks * (s.units + kPgSegCost);
+}
+
+// units per CTA: an equal share, and two groups a warp at least
 __device__ __forceinline__ long long pages_share(long long total, int ctas) {
-  const long long even = (total + ctas - 1) / ctas;
-  return even < 2 * kPgWarps ? 2 * kPgWarps : even;
+  const long long even = div_ll(total + ctas - 1, ctas);
+  return even < 2 * kPgWarps + kPgSegCost ? 2 * kPgWarps + kPgSegCost : even;
 }
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
@@ -116,57 +145,60 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// What a lane holds of one unit: K codes of two tokens, V codes of four.
-template <int D>
-struct PgUnit {
-  uint32_t k[2][D / 16];    // D / 4 bytes of tokens g and g + 8
-  uint32_t v[4][D / 32];    // D / 8 bytes of tokens 2t, 2t + 1, 2t + 8, 2t + 9
-  float2 scale;             // keys, values; NaN-free: an absent page is masked as a whole
-  bool present;
-};
-
-template <int D>
-__device__ __forceinline__ void load_unit(PgUnit<D>& u, const PagesParams& p, int entry, int g_head, int off, int lane) {
-  u.present = entry >= 0 && entry < p.P;
-  const long long block = (long long)(u.present ? entry : 0) * p.G + g_head;
-  const uint8_t* k = p.pool + ((block * 2) << p.log_page) * D + (long long)off * D;
-  const uint8_t* v = k + ((long long)D << p.log_page);
-  const int g = lane >> 2, t = lane & 3;
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int c = 0; c < D / 64; ++c) {
-      const uint4 x = ld_stream(k + (g + 8 * i) * D + t * (D / 4) + c * 16);
-      u.k[i][4 * c] = x.x; u.k[i][4 * c + 1] = x.y; u.k[i][4 * c + 2] = x.z; u.k[i][4 * c + 3] = x.w;
-    }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint8_t* src = v + (2 * t + (i & 1) + (i >> 1) * 8) * D + g * (D / 8);
-    if (D == 128) {
-      const uint4 x = ld_stream(src);
-      u.v[i][0] = x.x; u.v[i][1] = x.y; u.v[i][D / 32 - 2] = x.z; u.v[i][D / 32 - 1] = x.w;
-    } else {
-      asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(u.v[i][0]), "=r"(u.v[i][1]) : "l"(src));
-    }
-  }
-  u.scale = *reinterpret_cast<const float2*>(p.scales + block * 2);
-}
-
 // bit 7 of a byte set where the code is NaN (0x7f or 0xff)
 __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+
+// One segment's piece of a CTA's share.
+struct PagesPiece {
+  int b, gh, col0, cols;        // sequence, KV head, first query column, columns
+  int u_lo, u_hi;               // units of the segment
+  int first, last;              // units some column sees, within [u_lo, u_hi)
+  long long seg_at;             // where the segment begins in the dealt-out units
+};
+
 template <int D, int NT>
-__global__ void __launch_bounds__(kPgThreads, kPgCtasPerSm) mha_pages_kernel(const PagesParams p) {
+__global__ void __launch_bounds__(kPgThreads, kPgCtasPerSm)
+mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
   using Cfg = PgCfg<D, NT>;
-  constexpr int COLS = Cfg::kCols;
+  constexpr int COLS = Cfg::kCols, U = Cfg::kGroup;
   constexpr int KS = D / 16;                    // MMAs along d of a score
-  __shared__ float s_o[kPgWarps][COLS * D / 4];   // a quarter of d at a time
+  constexpr int NB = 32 / U;                    // groups whose pages a warp's lanes look up at once
+  extern __shared__ uint8_t pg_smem_raw[];
   __shared__ float s_m[kPgWarps][COLS], s_l[kPgWarps][COLS], s_w[kPgWarps][COLS];
-  __shared__ long long s_scan[kPgThreads];
-  __shared__ int s_b;
+  __shared__ long long s_scan[kPgWarps];
+  __shared__ int s_b, s_abort;
   __shared__ long long s_at;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pg_smem_raw) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int hg = p.H / p.G, page_mask = (1 << p.log_page) - 1;
+  const int hg = p.hg, page_mask = (1 << p.log_page) - 1;
+  float* s_o = reinterpret_cast<float*>(smem + Cfg::kMerge);   // [warp][column][D / kParts]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kBars) + warp * kPgStages;
+  const uint32_t ring = smem_u32(smem + Cfg::kRing) + warp * kPgStages * Cfg::kStage;
+  if (lane == 0) {
+    for (int i = 0; i < kPgStages; ++i) mbar_init(bars + i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (tid == 0) {
+    s_abort = 0;
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
+  }
 
   pdl_launch();
   pdl_wait();
@@ -176,78 +208,166 @@ __global__ void __launch_bounds__(kPgThreads, kPgCtasPerSm) mha_pages_kernel(con
   long long mine = 0;
   for (int b = sb; b < se; ++b) {
     const PagesSeq s = pages_seq<COLS>(p, b);
-    mine += (long long)s.segs * s.units;
+    mine += pages_cost(p, s);
   }
-  s_scan[tid] = mine;
+  long long before = mine, total = 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += x;
+  }
+  if (lane == 31) s_scan[warp] = before;
   __syncthreads();
-  long long before = 0, total = 0;
-  for (int i = 0; i < kPgThreads; ++i) {
-    const long long x = s_scan[i];
-    if (i < tid) before += x;
-    total += x;
+  before -= mine;
+#pragma unroll
+  for (int w = 0; w < kPgWarps; ++w) {
+    if (w < warp) before += s_scan[w];
+    total += s_scan[w];
   }
   const long long share = pages_share(total, p.ctas);
-  long long at = (long long)blockIdx.x * share;
-  const long long end = min(at + share, total);
-  if (at >= end) return;
-  if (at >= before && at < before + mine) {
+  const long long begin = (long long)blockIdx.x * share, end = min(begin + share, total);
+  if (tid == 0) p.records[blockIdx.x].pieces = 0;   // until this CTA begins a segment that others go on with
+  if (begin >= end) return;
+  if (begin >= before && begin < before + mine) {
     long long acc = before;
     for (int b = sb; b < se; ++b) {
       const PagesSeq s = pages_seq<COLS>(p, b);
-      const long long w = (long long)s.segs * s.units;
-      if (at < acc + w) { s_b = b; s_at = acc; break; }
+      const long long w = pages_cost(p, s);
+      if (begin < acc + w) { s_b = b; s_at = acc; break; }
       acc += w;
     }
   }
   __syncthreads();
-  int b = s_b;
-  long long seq_at = s_at;      // unit index where sequence b begins
-  PagesSeq seq = pages_seq<COLS>(p, b);
+  volatile int* abort_flag = &s_abort;
+  int seq_b = s_b;
+  long long seq_at = s_at;      // where sequence seq_b begins in the dealt-out units
+  PagesSeq seq = pages_seq<COLS>(p, seq_b);
 
-  while (at < end) {
-    while (at >= seq_at + (long long)seq.segs * seq.units) {
-      seq_at += (long long)seq.segs * seq.units;
-      seq = pages_seq<COLS>(p, ++b);
+  // The piece of the share [at, end) that begins at `at`; false when nothing is left.  A segment's
+  // units follow the kPgSegCost that it costs beside them, so a share may hold none of its own.
+  auto next_piece = [&](long long& at, PagesPiece& x) {
+    while (at < end) {
+      for (long long w; at >= seq_at + (w = pages_cost(p, seq));) {
+        seq_at += w;
+        seq = pages_seq<COLS>(p, ++seq_b);
+      }
+      const int span = seq.units + kPgSegCost;
+      const int seg = (int)div_ll(at - seq_at, span);
+      x.seg_at = seq_at + (long long)seg * span;
+      const int lo = (int)(at - x.seg_at), hi = (int)(min(end, x.seg_at + span) - x.seg_at);
+      at = x.seg_at + hi;
+      x.u_lo = max(lo - kPgSegCost, 0);
+      x.u_hi = max(hi - kPgSegCost, 0);
+      if (x.u_lo >= x.u_hi) continue;
+      x.b = seq_b;
+      x.gh = seq.blocks == 1 ? seg : seg / seq.blocks;
+      x.col0 = (seg - x.gh * seq.blocks) * COLS;
+      x.cols = min(COLS, seq.n * hg - x.col0);
+      int any_lo = 0, any_hi = seq.len;
+      const int past = seq.len - seq.n;
+      if (p.causal) any_hi = min(any_hi, past + (x.col0 + x.cols - 1) / hg + 1);
+      if (p.window >= 0) any_lo = max(0, past + x.col0 / hg - p.window);
+      x.first = max(x.u_lo, any_lo / kPgUnit - seq.unit0);
+      x.last = min(x.u_hi, (max(any_hi, 0) + kPgUnit - 1) / kPgUnit - seq.unit0);
+      return true;
     }
-    const int seg = (int)((at - seq_at) / seq.units);
-    const long long seg_at = seq_at + (long long)seg * seq.units;
-    const int u_lo = (int)(at - seg_at), u_hi = (int)(min(end, seg_at + seq.units) - seg_at);
-    const int blocks = seq.segs / p.G;
-    const int gh = seg / blocks, col0 = (seg % blocks) * COLS;
-    const int cols = min(COLS, seq.n * hg - col0);
-    const int past = seq.len - seq.n;           // position of the first row
-    const int* table = p.tables + (long long)b * p.width;
+    return false;
+  };
 
+  int filled = 0, drained = 0;   // groups of this warp so far: a group's stage and phase
+  // lane l looks up unit l % U of group l / U of a batch of NB groups
+  struct Batch { int entry; float sk, log_v, inv_v; };
+  auto look_up = [&](const PagesPiece& x, int unit0, int k0) {
+    const int u = x.first + ((k0 + lane / U) * kPgWarps + warp) * U + lane % U;
+    int e = -1;
+    if (u < x.last) e = p.tables[(long long)x.b * p.width + min(((unit0 + u) * kPgUnit) >> p.log_page, p.width - 1)];
+    return e >= 0 && e < p.P ? e : -1;
+  };
+  auto look_up_scales = [&](const PagesPiece& x, Batch& q) {
+    float2 s = make_float2(1.f, 1.f);
+    if (q.entry >= 0) s = *reinterpret_cast<const float2*>(p.scales + ((long long)q.entry * p.G + x.gh) * 2);
+    q.sk = s.x;
+    q.log_v = __log2f(s.y);
+    q.inv_v = 1.f / s.y;
+  };
+  // group k of the piece into the ring: lanes 0 .. U - 1 a unit each
+  auto fill = [&](const PagesPiece& x, int unit0, const Batch& q, int k) {
+    const int entry = __shfl_sync(0xffffffffu, q.entry, (k % NB) * U + (lane % U));
+    const int u = x.first + (k * kPgWarps + warp) * U + lane;
+    const bool on = lane < U && entry >= 0;
+    const int n = __popc(__ballot_sync(0xffffffffu, on));
+    const int stage = filled % kPgStages;
+    if (lane == 0) mbar_expect_tx(bars + stage, n * 2 * Cfg::kHalf);
+    __syncwarp();
+    if (on) {
+      const uint32_t dst = ring + stage * Cfg::kStage + lane * 2 * Cfg::kHalf, bar = smem_u32(bars + stage);
+      const int off = ((unit0 + u) * kPgUnit) & page_mask, block = entry * p.G + x.gh;
+      tma_load_3d(dst, &map, 0, off, block, bar);
+      tma_load_3d(dst + Cfg::kHalf, &map, 0, page_mask + 1 + off, block, bar);
+    }
+    ++filled;
+  };
+  auto groups_of = [&](const PagesPiece& x) {
+    const int units = x.last - x.first, groups = (max(units, 0) + U - 1) / U;
+    return (groups - warp + kPgWarps - 1) / kPgWarps;
+  };
+
+  long long at = begin;
+  PagesPiece cur;
+  PagesSeq cur_seq = seq;
+  Batch bat, bat_next;
+  uint4 q_raw[NT][D / 32];      // this lane's share of the queries of columns 8 nt + g: a run of D / 4
+  // the loads that a piece begins with, in the order in which others wait for them
+  auto open_piece = [&]() {
+    bat.entry = look_up(cur, cur_seq.unit0, 0);
+    bat_next.entry = look_up(cur, cur_seq.unit0, NB);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int c = nt * 8 + g;
+      const bool live = c < cur.cols;
+      const int row = live ? (cur.col0 + c) / hg : 0, h = live ? (cur.col0 + c) - row * hg : 0;
+      const __nv_bfloat16* src = p.q + ((long long)(cur_seq.row0 + row) * p.H + cur.gh * hg + h) * D + t * (D / 4);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) q_raw[nt][i] = live ? ld_cached(src + 8 * i) : make_uint4(0, 0, 0, 0);
+    }
+    const int n = groups_of(cur);
+    for (int k = 0; k < kPgStages && k < n; ++k) fill(cur, cur_seq.unit0, bat, k);
+    look_up_scales(cur, bat);
+    look_up_scales(cur, bat_next);
+  };
+  bool have = next_piece(at, cur);
+  cur_seq = seq;
+  bool ok = true;
+  if (have) {
+    open_piece();
+  }
+  while (have) {
+    const int past = cur_seq.len - cur_seq.n;     // position of the first row
+    const int len = cur_seq.len, unit0 = cur_seq.unit0;
     // ---- Q: this lane's share of column 8 nt + g, in halves under a power of two ----
     uint32_t qf[NT][KS][2];
     float colfac[NT][2];                        // of columns 8 nt + 2t and + 1
     int hi_key[NT][2], lo_key[NT][2];           // keys those columns see: [lo, hi)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int c = nt * 8 + g;
-      const bool live = c < cols;
-      const int row = live ? (col0 + c) / hg : 0, h = live ? (col0 + c) % hg : 0;
-      const __nv_bfloat16* src = p.q + ((long long)(seq.row0 + row) * p.H + gh * hg + h) * D + t * (D / 4);
-      uint4 raw[D / 32];
       float mx = 0.f;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
-        raw[i] = live ? ld_cached(src + 8 * i) : make_uint4(0, 0, 0, 0);
         float f[8];
-        unpack8(raw[i], f);
+        unpack8(q_raw[nt][i], f);
 #pragma unroll
         for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fabsf(f[j]));
       }
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       // mx * up lies in [2^14, 2^15); zero, subnormal and non-finite rows keep finite factors
-      const int e = min(max((int)(__float_as_uint(mx) >> 23), 1 + 14), 254);
-      const float up = __uint_as_float((uint32_t)(127 + 14 + 127 - e > 254 ? 254 : 127 + 14 + 127 - e) << 23);
+      const int e = min(max((int)(__float_as_uint(mx) >> 23), 15), 254);
+      const float up = __uint_as_float((uint32_t)(268 - e) << 23);
       const float down = 1.0f / up;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
         float f[8];
-        unpack8(raw[i], f);
+        unpack8(q_raw[nt][i], f);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           qf[nt][2 * i + j][0] = pack_half2(f[4 * j] * up, f[4 * j + 1] * up);
@@ -258,21 +378,14 @@ __global__ void __launch_bounds__(kPgThreads, kPgCtasPerSm) mha_pages_kernel(con
       for (int j = 0; j < 2; ++j) {
         colfac[nt][j] = __shfl_sync(0xffffffffu, down, (2 * t + j) * 4) * p.scale_log2;
         const int cc = nt * 8 + 2 * t + j;
-        const int pos = past + (col0 + min(cc, cols - 1)) / hg;
-        hi_key[nt][j] = cc < cols ? (p.causal ? min(seq.len, pos + 1) : seq.len) : 0;
+        const int pos = past + (cur.col0 + min(cc, cur.cols - 1)) / hg;
+        hi_key[nt][j] = cc < cur.cols ? (p.causal ? min(len, pos + 1) : len) : 0;
         lo_key[nt][j] = p.window >= 0 ? pos - p.window : 0;
       }
     }
-    // the keys every column sees, and any column sees
-    int all_hi = seq.len, any_hi = seq.len, all_lo = 0, any_lo = 0;
-    if (p.causal) {
-      all_hi = min(seq.len, past + col0 / hg + 1);
-      any_hi = min(seq.len, past + (col0 + cols - 1) / hg + 1);
-    }
-    if (p.window >= 0) {
-      any_lo = past + col0 / hg - p.window;
-      all_lo = past + (col0 + cols - 1) / hg - p.window;
-    }
+    // the keys that every column sees
+    const int all_hi = p.causal ? min(len, past + cur.col0 / hg + 1) : len;
+    const int all_lo = p.window >= 0 ? past + (cur.col0 + cur.cols - 1) / hg - p.window : 0;
 
     float o[KS][NT][4], m_run[NT][2], l_run[NT][2];
 #pragma unroll
@@ -285,81 +398,131 @@ __global__ void __launch_bounds__(kPgThreads, kPgCtasPerSm) mha_pages_kernel(con
         for (int j = 0; j < 4; ++j) o[i][nt][j] = 0.f;
     }
 
-    // units any column sees; the rest of the run is masked as a whole
-    const int first = max(u_lo, max(any_lo, 0) / kPgUnit - seq.unit0);
-    const int last = min(u_hi, (any_hi + kPgUnit - 1) / kPgUnit - seq.unit0);
-    auto entry_of = [&](int u) {
-      return u < last ? table[min(((seq.unit0 + u) * kPgUnit) >> p.log_page, p.width - 1)] : -1;
-    };
-    int u = first + warp;
-    PgUnit<D> cur;
-    int entry = entry_of(u);
-    if (u < last) load_unit<D>(cur, p, entry, gh, ((seq.unit0 + u) * kPgUnit) & page_mask, lane);
-    entry = entry_of(u + kPgWarps);
-    for (; u < last; u += kPgWarps) {
-      PgUnit<D> nxt;
-      if (u + kPgWarps < last)
-        load_unit<D>(nxt, p, entry, gh, ((seq.unit0 + u + kPgWarps) * kPgUnit) & page_mask, lane);
-      entry = entry_of(u + 2 * kPgWarps);
-      const int tok0 = (seq.unit0 + u) * kPgUnit;
-      if (cur.present) {
-        // ---- S^T = K Q^T ----
-        float s[NT][4];
+    const int groups = groups_of(cur);
+    for (int k = 0; k < groups && ok; ++k) {
+      const int stage = drained % kPgStages;
+      ok = mbar_wait(bars + stage, (drained / kPgStages) & 1, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      ++drained;
+      const uint32_t base = ring + stage * Cfg::kStage;
+      const int src0 = (k % NB) * U;
+      // ---- S^T = K Q^T ----
+      float s[U][NT][4];
+      bool whole[U], present[U];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+      for (int i = 0; i < U; ++i) {
+        present[i] = __shfl_sync(0xffffffffu, bat.entry, src0 + i) >= 0;
+        const float sk = __shfl_sync(0xffffffffu, bat.sk, src0 + i), lv = __shfl_sync(0xffffffffu, bat.log_v, src0 + i);
+        const int tok0 = (unit0 + cur.first + (k * kPgWarps + warp) * U + i) * kPgUnit;
+        whole[i] = present[i] && tok0 + kPgUnit <= all_hi && tok0 >= all_lo;
+        uint32_t kf[2][D / 16];
+        const uint32_t kb = base + i * 2 * Cfg::kHalf;
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-          const uint32_t a[4] = {e4m3x2_to_half2(cur.k[0][i]), e4m3x2_to_half2(cur.k[1][i]),
-                                 e4m3x2_to_half2(cur.k[0][i] >> 16), e4m3x2_to_half2(cur.k[1][i] >> 16)};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_f16_16816(s[nt], a, qf[nt][i][0], qf[nt][i][1]);
+        for (int r = 0; r < 2; ++r) {
+          if (D == 128) {
+            const uint32_t row = kb + (g + 8 * r) * 128;
+            const uint4 x = lds128(row + (((2 * t) ^ g) << 4)), y = lds128(row + (((2 * t + 1) ^ g) << 4));
+            kf[r][0] = x.x; kf[r][1] = x.y; kf[r][2] = x.z; kf[r][3] = x.w;
+            kf[r][D / 16 - 4] = y.x; kf[r][D / 16 - 3] = y.y; kf[r][D / 16 - 2] = y.z; kf[r][D / 16 - 1] = y.w;
+          } else {
+            const uint4 x = lds128(kb + (g + 8 * r) * 64 + ((t ^ ((g >> 1) & 3)) << 4));
+            kf[r][0] = x.x; kf[r][1] = x.y; kf[r][2] = x.z; kf[r][3] = x.w;
+          }
         }
-        const bool whole = tok0 + kPgUnit <= all_hi && tok0 >= all_lo;
-        const float log_v = __log2f(cur.scale.y), inv_v = 1.f / cur.scale.y;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) s[i][nt][0] = s[i][nt][1] = s[i][nt][2] = s[i][nt][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < KS; ++c) {
+          const uint32_t a[4] = {e4m3x2_to_half2(kf[0][c]), e4m3x2_to_half2(kf[1][c]),
+                                 e4m3x2_to_half2(kf[0][c] >> 16), e4m3x2_to_half2(kf[1][c] >> 16)};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16_16816(s[i][nt], a, qf[nt][c][0], qf[nt][c][1]);
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            s[nt][j] = fmaf(s[nt][j], colfac[nt][j & 1] * cur.scale.x, log_v);
-            if (!whole) {
+          for (int j = 0; j < 4; ++j) s[i][nt][j] = fmaf(s[i][nt][j], colfac[nt][j & 1] * sk, lv);
+        if (!whole[i]) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
               const int key = tok0 + g + (j >> 1) * 8;
-              if (key >= hi_key[nt][j & 1] || key < lo_key[nt][j & 1]) s[nt][j] = -INFINITY;
+              if (!present[i] || key >= hi_key[nt][j & 1] || key < lo_key[nt][j & 1]) s[i][nt][j] = -INFINITY;
             }
+        }
+      }
+      // ---- running maximum and sum ----
+      float m_new[NT][2];
+      bool moved = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float m = fmaxf(s[0][nt][j], s[0][nt][j + 2]);
+#pragma unroll
+          for (int i = 1; i < U; ++i) m = fmaxf(m, fmaxf(s[i][nt][j], s[i][nt][j + 2]));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+          m_new[nt][j] = fmaxf(m_run[nt][j], m);
+          moved = moved || m_new[nt][j] != m_run[nt][j];
+        }
+      if (__any_sync(0xffffffffu, moved)) {   // seldom after the first groups
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float corr = ex2(m_run[nt][j] - (m_new[nt][j] == -INFINITY ? 0.f : m_new[nt][j]));
+            m_run[nt][j] = m_new[nt][j];
+            l_run[nt][j] *= corr;
+#pragma unroll
+            for (int i = 0; i < KS; ++i) { o[i][nt][j] *= corr; o[i][nt][j + 2] *= corr; }
           }
-        // ---- running maximum and sum ----
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        if (!present[i]) continue;              // the stage holds nothing there
+        const float inv_v = __shfl_sync(0xffffffffu, bat.inv_v, src0 + i);
         uint32_t pb[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float pr[4];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float m = fmaxf(s[nt][j], s[nt][j + 2]);
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-            const float m_new = fmaxf(m_run[nt][j], m);
-            const float safe = m_new == -INFINITY ? 0.f : m_new;
-            const float corr = ex2(m_run[nt][j] - safe);
-            m_run[nt][j] = m_new;
-            pr[j] = ex2(s[nt][j] - safe + kPgLift);
-            pr[j + 2] = ex2(s[nt][j + 2] - safe + kPgLift);
-            l_run[nt][j] = l_run[nt][j] * corr + (pr[j] + pr[j + 2]) * inv_v;
-#pragma unroll
-            for (int i = 0; i < KS; ++i) { o[i][nt][j] *= corr; o[i][nt][j + 2] *= corr; }
+            const float zero = (m_run[nt][j] == -INFINITY ? 0.f : m_run[nt][j]) - kPgLift;
+            pr[j] = ex2(s[i][nt][j] - zero);
+            pr[j + 2] = ex2(s[i][nt][j + 2] - zero);
+            l_run[nt][j] = fmaf(pr[j] + pr[j + 2], inv_v, l_run[nt][j]);
           }
           pb[nt][0] = movmatrix_trans(pack_half2(pr[0], pr[1]));
           pb[nt][1] = movmatrix_trans(pack_half2(pr[2], pr[3]));
         }
+        uint32_t vf[4][D / 32];
+        const uint32_t vb = base + i * 2 * Cfg::kHalf + Cfg::kHalf;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = 2 * t + (r & 1) + (r >> 1) * 8;
+          if (D == 128) {
+            const uint4 x = lds128(vb + row * 128 + ((g ^ (row & 7)) << 4));
+            vf[r][0] = x.x; vf[r][1] = x.y; vf[r][D / 32 - 2] = x.z; vf[r][D / 32 - 1] = x.w;
+          } else {
+            const uint2 x = lds64(vb + row * 64 + ((((g >> 1) ^ ((row >> 1) & 3)) << 4) | ((g & 1) << 3)));
+            vf[r][0] = x.x; vf[r][1] = x.y;
+          }
+        }
         // ---- a NaN value of a token some column does not see must not reach it through 0 x NaN ----
-        if (!whole) {
+        if (!whole[i]) {
           uint32_t bad = 0;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int w = 0; w < D / 32; ++w) bad |= nan_codes(cur.v[i][w]);
+            for (int w = 0; w < D / 32; ++w) bad |= nan_codes(vf[r][w]);
           if (__any_sync(0xffffffffu, bad != 0)) {
             // NaN codes become zeros; where a column sees one, its output becomes NaN: the counts
             // of (NaN, seen) pairs are a product of the same shape
+            const int tok0 = (unit0 + cur.first + (k * kPgWarps + warp) * U + i) * kPgUnit;
             uint32_t seen[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -371,13 +534,13 @@ __global__ void __launch_bounds__(kPgThreads, kPgCtasPerSm) mha_pages_kernel(con
                 seen[nt][h] = movmatrix_trans((s0 ? 0x3c00u : 0u) | (s1 ? 0x3c000000u : 0u));
               }
 #pragma unroll
-            for (int i = 0; i < KS; ++i) {
-              const int w = i >> 1, sh = 16 * (i & 1);
+            for (int c = 0; c < KS; ++c) {
+              const int w = c >> 1, sh = 16 * (c & 1);
               uint32_t a[4];
 #pragma unroll
               for (int r = 0; r < 4; ++r) {      // a0: byte 0 of tokens 0, 1; a1: byte 1; a2, a3: tokens 2, 3
-                const uint32_t x = nan_codes(cur.v[(r >> 1) * 2][w]) >> (sh + 8 * (r & 1) + 7);
-                const uint32_t y = nan_codes(cur.v[(r >> 1) * 2 + 1][w]) >> (sh + 8 * (r & 1) + 7);
+                const uint32_t x = nan_codes(vf[(r >> 1) * 2][w]) >> (sh + 8 * (r & 1) + 7);
+                const uint32_t y = nan_codes(vf[(r >> 1) * 2 + 1][w]) >> (sh + 8 * (r & 1) + 7);
                 a[r] = ((x & 1u) ? 0x3c00u : 0u) | ((y & 1u) ? 0x3c000000u : 0u);
               }
 #pragma unroll
@@ -386,26 +549,43 @@ __global__ void __launch_bounds__(kPgThreads, kPgCtasPerSm) mha_pages_kernel(con
                 mma_f16_16816(n, a, seen[nt][0], seen[nt][1]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                  if (n[j] > 0.f) o[i][nt][j] = __uint_as_float(0x7fc00000u);
+                  if (n[j] > 0.f) o[c][nt][j] = __uint_as_float(0x7fc00000u);
               }
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int r = 0; r < 4; ++r)
 #pragma unroll
-              for (int w = 0; w < D / 32; ++w) cur.v[i][w] &= ~((nan_codes(cur.v[i][w]) >> 7) * 0xffu);
+              for (int w = 0; w < D / 32; ++w) vf[r][w] &= ~((nan_codes(vf[r][w]) >> 7) * 0xffu);
           }
         }
         // ---- O^T += V^T P^T ----
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-          const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;
-          const uint32_t x = prmt(cur.v[0][i >> 1], cur.v[1][i >> 1], sel), y = prmt(cur.v[2][i >> 1], cur.v[3][i >> 1], sel);
+        for (int c = 0; c < KS; ++c) {
+          const uint32_t sel = (c & 1) ? 0x7362u : 0x5140u;
+          const uint32_t x = prmt(vf[0][c >> 1], vf[1][c >> 1], sel), y = prmt(vf[2][c >> 1], vf[3][c >> 1], sel);
           const uint32_t a[4] = {e4m3x2_to_half2(x), e4m3x2_to_half2(x >> 16), e4m3x2_to_half2(y), e4m3x2_to_half2(y >> 16)};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_f16_16816(o[i][nt], a, pb[nt][0], pb[nt][1]);
+          for (int nt = 0; nt < NT; ++nt) mma_f16_16816(o[c][nt], a, pb[nt][0], pb[nt][1]);
         }
       }
-      cur = nxt;
+      // ---- the stage is read: the group kPgStages on takes it ----
+      __syncwarp();
+      const int kf_ = k + kPgStages;
+      if (kf_ < groups) fill(cur, unit0, kf_ / NB == k / NB ? bat : bat_next, kf_);
+      if ((k + 1) % NB == 0) {
+        bat = bat_next;
+        bat_next.entry = look_up(cur, unit0, k + 1 + NB);
+        look_up_scales(cur, bat_next);
+      }
+    }
+
+    // the next piece's first groups come while this one's results meet
+    const PagesPiece done = cur;
+    const PagesSeq done_seq = cur_seq;
+    have = ok && next_piece(at, cur);
+    cur_seq = seq;
+    if (have) {
+      open_piece();
     }
 
     // ---- the warps' results meet; a lane's sums are of its own tokens only ----
@@ -431,116 +611,180 @@ __global__ void __launch_bounds__(kPgThreads, kPgCtasPerSm) mha_pages_kernel(con
       }
       s_m[0][tid] = m; s_l[0][tid] = l;
     }
-    const bool direct = u_lo == 0 && u_hi == seq.units;
-    // a run that begins before this CTA's share uses the CTA's first slot, one that goes on the second
-    float* part = p.partial + ((long long)blockIdx.x * 2 + (u_lo == 0 ? 1 : 0)) * Cfg::kPartial;
+    const bool direct = done.u_lo == 0 && done.u_hi == done_seq.units;
+    // a piece that begins before this CTA's share uses the CTA's first slot, one that goes on the second
+    float* part = p.partial + ((long long)blockIdx.x * 2 + (done.u_lo == 0 ? 1 : 0)) * Cfg::kPartial;
+    // the outputs meet a part of d at a time: MMA c holds codes 2 c and 2 c + 1 of each lane
+    // group's run of D / 8
+    constexpr int kParts = Cfg::kParts, CP = KS / kParts, DP = D / kParts;
 #pragma unroll
-    for (int quarter = 0; quarter < 4; ++quarter) {
-      __syncthreads();
-      // rows of O^T in MMA i: codes 2 i and 2 i + 1 of each lane group's run of D / 8
+    for (int part_i = 0; part_i < kParts; ++part_i) {
+      if (part_i) __syncthreads();
 #pragma unroll
-      for (int i = quarter * KS / 4; i < (quarter + 1) * KS / 4; ++i)
+      for (int c = part_i * CP; c < (part_i + 1) * CP; ++c)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int c = nt * 8 + 2 * t + (j & 1);
-            const int dd = g * (D / 32) + 2 * (i - quarter * KS / 4) + (j >> 1);   // of this quarter
-            s_o[warp][c * (D / 4) + dd] = o[i][nt][j];
+            const int col = nt * 8 + 2 * t + (j & 1);
+            const int dd = g * (2 * CP) + 2 * (c - part_i * CP) + (j >> 1);   // of this part
+            s_o[(warp * COLS + col) * DP + dd] = o[c][nt][j];
           }
       __syncthreads();
-      for (int x = tid; x < cols * (D / 4); x += kPgThreads) {
-        const int c = x / (D / 4), dd = x % (D / 4);
-        const int d = (dd / (D / 32)) * (D / 8) + quarter * (D / 32) + dd % (D / 32);
+      for (int x = tid; x < done.cols * DP; x += kPgThreads) {
+        const int col = x / DP, dd = x % DP;
+        const int d = (dd / (2 * CP)) * (D / 8) + part_i * 2 * CP + dd % (2 * CP);
         float acc = 0.f;
 #pragma unroll
-        for (int w = 0; w < kPgWarps; ++w) acc += s_o[w][c * (D / 4) + dd] * s_w[w][c];
+        for (int w = 0; w < kPgWarps; ++w) acc += s_o[(w * COLS + col) * DP + dd] * s_w[w][col];
         if (direct) {
-          const float l = s_l[0][c];
-          const int row = (col0 + c) / hg, h = (col0 + c) % hg;
+          const float l = s_l[0][col];
+          const int row = (done.col0 + col) / hg, h = (done.col0 + col) % hg;
           // a row that sees nothing is zero; l is NaN where a score it sees is
-          p.out[((long long)(seq.row0 + row) * p.H + gh * hg + h) * D + d] = __float2bfloat16_rn(l == 0.f ? 0.f : acc / l);
+          p.out[((long long)(done_seq.row0 + row) * p.H + done.gh * hg + h) * D + d] =
+              __float2bfloat16_rn(l == 0.f ? 0.f : acc / l);
         } else {
-          part[c * D + d] = acc;
+          part[col * D + d] = acc;
         }
       }
     }
-    if (!direct && tid < cols) {
-      part[COLS * D + tid] = s_m[0][tid];
-      part[COLS * D + COLS + tid] = s_l[0][tid];
+    if (!direct) {
+      if (tid == 0 && done.u_lo == 0) {
+        const long long seg_end = done.seg_at + done_seq.units + kPgSegCost;
+        PagesRecord r;
+        r.pieces = (int)((seg_end - 1) / share) - (int)blockIdx.x + 1;
+        r.row0 = done_seq.row0; r.head0 = done.gh * hg; r.col0 = done.col0;
+        r.cols = done.cols;
+        p.records[blockIdx.x] = r;
+      }
+      if (tid < done.cols) {
+        part[COLS * D + tid] = s_m[0][tid];
+        part[COLS * D + COLS + tid] = s_l[0][tid];
+      }
     }
-    __syncthreads();   // shared memory is the next run's
-    at = seg_at + u_hi;
+    __syncthreads();   // shared memory is the next piece's
+    ok = ok && !*abort_flag;
+    have = have && ok;
+  }
+  if (!ok) {
+    // a wait gave up: give the copies in flight a millisecond, many times what one takes
+    if (tid == 0 && p.status) *p.status = IRON_ERR_TIMEOUT;
+    const unsigned long long t0 = global_ns();
+    while (global_ns() - t0 < 1000000ull) {}
   }
 }
 
-// Folds the partials of cut segments, in the order of their keys.  One CTA a sequence (and a KV
-// head); a segment that one CTA held whole was written by it.
+// Folds the partials of a segment that several CTAs share, in the order of its keys.  One CTA for
+// each main CTA, whose record says whether it begins such a segment, and column; the warps take the
+// pieces in turn, a lane a stretch of d.
+constexpr int kFoldWarps = 8;
+constexpr int kFoldBatch = 4;    // pieces whose loads a warp has in flight at once
 template <int D, int NT>
-__global__ void __launch_bounds__(kPgThreads) mha_pages_fold_kernel(const PagesParams p) {
+__global__ void __launch_bounds__(kFoldWarps * 32) mha_pages_fold_kernel(const PagesParams p) {
   using Cfg = PgCfg<D, NT>;
-  constexpr int COLS = Cfg::kCols;
-  __shared__ long long s_sum[2 * kPgWarps];
-  __shared__ float s_f[kPgCtas];
+  constexpr int COLS = Cfg::kCols, PER = D / 32;
+  __shared__ float s_o[kFoldWarps][D], s_m[kFoldWarps], s_l[kFoldWarps];
   pdl_launch();
   pdl_wait();
-  const int b = blockIdx.x, gh = blockIdx.y, tid = threadIdx.x, hg = p.H / p.G;
-  long long before = 0, total = 0;
-  for (int i = tid; i < p.B; i += kPgThreads) {
-    const PagesSeq s = pages_seq<COLS>(p, i);
-    const long long w = (long long)s.segs * s.units;
-    total += w;
-    if (i < b) before += w;
-  }
+  const PagesRecord r = p.records[blockIdx.x];
+  const int c = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (r.pieces <= 1 || c >= r.cols) return;
+  float m = -INFINITY, l = 0.f, o[PER];
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-    total += __shfl_xor_sync(0xffffffffu, total, o);
-  }
-  if ((tid & 31) == 0) { s_sum[2 * (tid >> 5)] = before; s_sum[2 * (tid >> 5) + 1] = total; }
-  __syncthreads();
-  before = total = 0;
-  for (int w = 0; w < kPgWarps; ++w) { before += s_sum[2 * w]; total += s_sum[2 * w + 1]; }
-  const PagesSeq seq = pages_seq<COLS>(p, b);
-  const long long share = pages_share(total, p.ctas);
-  const int blocks = seq.segs / p.G;
-  for (int cb = 0; cb < blocks; ++cb) {
-    const long long s0 = before + ((long long)gh * blocks + cb) * seq.units, s1 = s0 + seq.units;
-    const int c_lo = (int)(s0 / share), c_hi = (int)((s1 - 1) / share), pieces = c_hi - c_lo + 1;
-    if (pieces == 1) continue;
-    const int col0 = cb * COLS, cols = min(COLS, seq.n * hg - col0);
-    // the piece that begins the segment lies in its CTA's second slot, the others in the first
-    auto slot_of = [&](int i) { return p.partial + ((long long)(c_lo + i) * 2 + (i == 0 ? 1 : 0)) * Cfg::kPartial; };
-    for (int c = 0; c < cols; ++c) {
-      __syncthreads();
-      float m = -INFINITY;
-      for (int i = 0; i < pieces; ++i) m = fmaxf(m, slot_of(i)[COLS * D + c]);
-      const float safe = m == -INFINITY ? 0.f : m;
-      for (int i = tid; i < pieces; i += kPgThreads) s_f[i] = ex2(slot_of(i)[COLS * D + c] - safe);
-      __syncthreads();
-      if (tid < D) {
-        float l = 0.f, acc = 0.f;
-        for (int i = 0; i < pieces; ++i) {
-          l += slot_of(i)[COLS * D + COLS + c] * s_f[i];
-          acc += slot_of(i)[c * D + tid] * s_f[i];
-        }
-        const int row = (col0 + c) / hg, h = (col0 + c) % hg;
-        p.out[((long long)(seq.row0 + row) * p.H + gh * hg + h) * D + tid] = __float2bfloat16_rn(l == 0.f ? 0.f : acc / l);
-      }
+  for (int j = 0; j < PER; ++j) o[j] = 0.f;
+  for (int i0 = warp; i0 < r.pieces; i0 += kFoldBatch * kFoldWarps) {
+    float x[kFoldBatch][PER], mi[kFoldBatch], li[kFoldBatch];
+#pragma unroll
+    for (int k = 0; k < kFoldBatch; ++k) {
+      const int i = min(i0 + k * kFoldWarps, r.pieces - 1);   // past the end: loaded again, not counted
+      // the piece that begins the segment lies in its CTA's second slot, the others in the first
+      const float* src = p.partial + ((long long)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * Cfg::kPartial;
+      mi[k] = src[COLS * D + c];
+      li[k] = src[COLS * D + COLS + c];
+      const float2* v = reinterpret_cast<const float2*>(src + c * D + lane * PER);
+#pragma unroll
+      for (int j = 0; j < PER / 2; ++j) { const float2 y = v[j]; x[k][2 * j] = y.x; x[k][2 * j + 1] = y.y; }
+    }
+#pragma unroll
+    for (int k = 0; k < kFoldBatch; ++k) {
+      if (i0 + k * kFoldWarps >= r.pieces) break;
+      const float m_new = fmaxf(m, mi[k]), safe = m_new == -INFINITY ? 0.f : m_new;
+      const float f = ex2(m - safe), fi = ex2(mi[k] - safe);
+      m = m_new;
+      l = l * f + li[k] * fi;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) o[j] = o[j] * f + x[k][j] * fi;
     }
   }
+#pragma unroll
+  for (int j = 0; j < PER; ++j) s_o[warp][lane * PER + j] = o[j];
+  if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
+  __syncthreads();
+  const int d = threadIdx.x, warps = min(kFoldWarps, r.pieces);
+  if (d < D) {
+    m = s_m[0];
+    for (int w = 1; w < warps; ++w) m = fmaxf(m, s_m[w]);
+    const float safe = m == -INFINITY ? 0.f : m;
+    float acc = 0.f;
+    l = 0.f;
+    for (int w = 0; w < warps; ++w) {
+      const float f = ex2(s_m[w] - safe);
+      l += s_l[w] * f;
+      acc += s_o[w][d] * f;
+    }
+    const int row = (r.col0 + c) / p.hg, h = (r.col0 + c) - row * p.hg;
+    p.out[((long long)(r.row0 + row) * p.H + r.head0 + h) * D + d] = __float2bfloat16_rn(l == 0.f ? 0.f : acc / l);
+  }
+}
+
+typedef CUresult (*PgEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                               const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// (byte of a row, row of a (page, head)'s keys and values, page x head); boxes of 16 whole rows.
+static bool pages_map(CUtensorMap* map, const PagesParams& p, int D) {
+  static std::atomic<PgEncodeFn> known{nullptr};
+  PgEncodeFn fn = known.load(std::memory_order_acquire);
+  if (!fn) {
+    void* sym = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return false;
+    fn = reinterpret_cast<PgEncodeFn>(sym);
+    known.store(fn, std::memory_order_release);
+  }
+  const cuuint64_t rows = (cuuint64_t)2 << p.log_page;
+  const cuuint64_t dims[3] = {(cuuint64_t)D, rows, (cuuint64_t)p.P * p.G};
+  const cuuint64_t strides[2] = {(cuuint64_t)D, (cuuint64_t)D * rows};
+  const cuuint32_t box[3] = {(cuuint32_t)D, (cuuint32_t)kPgUnit, 1}, elem[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(p.pool), dims, strides, box, elem,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int D, int NT>
 static int launch_pages(const PagesParams& p, cudaStream_t stream) {
+  CUtensorMap map;
+  if (!pages_map(&map, p, D)) return IRON_ERR_UNSUPPORTED;
+  constexpr int smem = PgCfg<D, NT>::kSmem;
+  static DeviceOnce configured;
+  if (!configured.done()) {
+    if (cudaFuncSetAttribute(mha_pages_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+      return IRON_ERR_LAUNCH;
+    configured.mark();
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kPgThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   fill_pdl_attr(cfg, attr);
   cfg.gridDim = dim3(p.ctas);
-  if (cudaLaunchKernelEx(&cfg, mha_pages_kernel<D, NT>, p) != cudaSuccess) return IRON_ERR_LAUNCH;
-  cfg.gridDim = dim3(p.B, p.G);
+  if (cudaLaunchKernelEx(&cfg, mha_pages_kernel<D, NT>, map, p) != cudaSuccess) return IRON_ERR_LAUNCH;
+  cfg.gridDim = dim3(p.ctas, p.row_start || NT * 8 < p.hg ? NT * 8 : p.hg);
+  cfg.blockDim = dim3(kFoldWarps * 32);
+  cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, mha_pages_fold_kernel<D, NT>, p) == cudaSuccess ? IRON_OK : IRON_ERR_LAUNCH;
 }
 
@@ -556,7 +800,7 @@ using namespace iron;
 extern "C" long long iron_mha_pages_workspace_bytes(int D) {
   if (D != 64 && D != 128) return 0;
   const long long partial = 16ll * D + 32;
-  return (long long)kPgCtas * 2 * partial * sizeof(float);
+  return (long long)kPgCtas * (2 * partial * (long long)sizeof(float) + (long long)sizeof(PagesRecord));
 }
 
 static int pages_args(PagesParams& p, const void* q, const void* pool, const float* scales, int P, int page_size,
@@ -566,7 +810,7 @@ static int pages_args(PagesParams& p, const void* q, const void* pool, const flo
   const int log_page = log2_page(page_size);
   if (B < 0 || rows < 0 || H <= 0 || G <= 0 || H % G || (D != 64 && D != 128) || P <= 0 || width <= 0 || log_page < 0)
     return IRON_ERR_SHAPE;
-  if (G > 65535 || (long long)P * page_size > 0x7fffffffll || (long long)rows * H > 0x7fffffffll) return IRON_ERR_SHAPE;
+  if (G > 65535 || (long long)P * G > 0x7fffffffll || (long long)P * page_size > 0x7fffffffll || (long long)rows * H > 0x7fffffffll) return IRON_ERR_SHAPE;
   if ((long long)width * page_size > 0x7fffffffll) return IRON_ERR_SHAPE;
   if (window >= 0 && !causal) return IRON_ERR_UNSUPPORTED;
   if (!(scale > 0.f)) return IRON_ERR_SHAPE;
@@ -577,8 +821,9 @@ static int pages_args(PagesParams& p, const void* q, const void* pool, const flo
     return IRON_ERR_ALIGN;
   if (workspace_bytes < iron_mha_pages_workspace_bytes(D)) return IRON_ERR_WORKSPACE;
   p.q = (const __nv_bfloat16*)q; p.pool = (const uint8_t*)pool; p.scales = scales; p.tables = tables;
-  p.lengths = lengths; p.row_start = row_start; p.out = (__nv_bfloat16*)out; p.partial = (float*)workspace;
-  p.B = B; p.H = H; p.G = G; p.P = P; p.width = width; p.log_page = log_page; p.causal = causal; p.window = window;
+  p.lengths = lengths; p.row_start = row_start; p.out = (__nv_bfloat16*)out; p.records = (PagesRecord*)workspace;
+  p.partial = (float*)(p.records + kPgCtas);
+  p.B = B; p.H = H; p.G = G; p.hg = H / G; p.P = P; p.width = width; p.log_page = log_page; p.causal = causal; p.window = window;
   p.rows = rows; p.ctas = kPgCtas;
   p.scale_log2 = scale * 1.4426950408889634f;
   return IRON_OK;
@@ -587,22 +832,24 @@ static int pages_args(PagesParams& p, const void* q, const void* pool, const flo
 extern "C" int iron_mha_decode_pages_bf16(const void* q, const void* pool, const float* scales, int P, int page_size,
                                           const int* tables, int width, const int* lengths, int B, int H, int G, int D,
                                           int window, float scale, void* workspace, long long workspace_bytes, void* out,
-                                          iron_stream_t stream) {
+                                          int* status, iron_stream_t stream) {
   PagesParams p = {};
   const int rc = pages_args(p, q, pool, scales, P, page_size, tables, width, lengths, nullptr, B, B, H, G, D, 1, window,
                             scale, workspace, workspace_bytes, out);
   if (rc) return rc == 1 ? IRON_OK : rc;
+  p.status = status;
   return D == 64 ? launch_pages_cols<64>(p, H / G, (cudaStream_t)stream) : launch_pages_cols<128>(p, H / G, (cudaStream_t)stream);
 }
 
 extern "C" int iron_mha_prefill_pages_bf16(const void* q, const void* pool, const float* scales, int P, int page_size,
                                            const int* tables, int width, const int* lengths, const int* row_start, int B,
                                            int rows, int H, int G, int D, int causal, int window, float scale,
-                                           void* workspace, long long workspace_bytes, void* out, iron_stream_t stream) {
+                                           void* workspace, long long workspace_bytes, void* out, int* status, iron_stream_t stream) {
   PagesParams p = {};
   const int rc = pages_args(p, q, pool, scales, P, page_size, tables, width, lengths, row_start, B, rows, H, G, D,
                             causal, window, scale, workspace, workspace_bytes, out);
   if (rc) return rc == 1 ? IRON_OK : rc;
+  p.status = status;
   if (!row_start) return IRON_ERR_SHAPE;
   return D == 64 ? launch_pages<64, 2>(p, (cudaStream_t)stream) : launch_pages<128, 2>(p, (cudaStream_t)stream);
 }

@@ -687,23 +687,25 @@ def _pages_attention(Q, pool, scales, tables, lengths, out, workspace):
     return P, G, page, D, out, workspace
 
 
-def mha_decode_pages(Q, pool, scales, tables, lengths, out=None, *, window=None, scale=None, workspace=None):
+def mha_decode_pages(Q, pool, scales, tables, lengths, out=None, *, window=None, scale=None, workspace=None,
+                     status=None):
     """One query a request, ``Q`` (B, H, D), over the paged cache's first ``lengths[b]`` tokens.
 
     ``window`` keeps the keys within that many positions of the last.  ``workspace``:
-    ``pages_workspace``'s buffer, allocated for the call when not given."""
+    ``pages_workspace``'s buffer, allocated for the call when not given; ``status``: an int32 word
+    that receives ``IRON_ERR_TIMEOUT`` when a bounded wait gives up."""
     if Q.shape[:1] != lengths.shape:
         raise ValueError(f"Q {tuple(Q.shape)} is not one query for each of {tuple(lengths.shape)} requests")
     P, G, page, D, out, workspace = _pages_attention(Q, pool, scales, tables, lengths, out, workspace)
     call("iron_mha_decode_pages_bf16", Q.data_ptr(), pool.data_ptr(), scales.data_ptr(), P, page, tables.data_ptr(),
          tables.shape[1], lengths.data_ptr(), Q.shape[0], Q.shape[1], G, D, -1 if window is None else int(window),
          1.0 / math.sqrt(D) if scale is None else float(scale), workspace.data_ptr(), workspace.numel(),
-         out.data_ptr(), _stream())
+         out.data_ptr(), _ptr(status), _stream())
     return out
 
 
 def mha_prefill_pages(Q, pool, scales, tables, lengths, row_start, out=None, *, causal=True, window=None, scale=None,
-                      workspace=None):
+                      workspace=None, status=None):
     """Ragged query rows over the paged cache: request ``b``'s are ``Q[row_start[b]:row_start[b + 1]]``,
     at the last positions of its ``lengths[b]`` tokens.
 
@@ -720,7 +722,7 @@ def mha_prefill_pages(Q, pool, scales, tables, lengths, row_start, out=None, *, 
     call("iron_mha_prefill_pages_bf16", Q.data_ptr(), pool.data_ptr(), scales.data_ptr(), P, page, tables.data_ptr(),
          tables.shape[1], lengths.data_ptr(), row_start.data_ptr(), B, Q.shape[0], Q.shape[1], G, D, int(bool(causal)),
          -1 if window is None else int(window), 1.0 / math.sqrt(D) if scale is None else float(scale),
-         workspace.data_ptr(), workspace.numel(), out.data_ptr(), _stream())
+         workspace.data_ptr(), workspace.numel(), out.data_ptr(), _ptr(status), _stream())
     return out
 
 

@@ -116,13 +116,13 @@ def test_the_c_entries_refuse_before_any_launch():
 
     def attend(H=4, G=2, D=64, B=2, rows=2, page=16, causal=1, window=-1, scale=1.0, q=a, starts=a, nbytes=1 << 40):
         return lib.iron_mha_prefill_pages_bf16(q, a, a, 4, page, a, 1, a, starts, B, rows, H, G, D, causal, window, scale,
-                                               a, nbytes, a, None)
+                                               a, nbytes, a, None, None)
 
     assert attend(H=5) == attend(D=80) == attend(page=17) == attend(scale=0.0) == attend(scale=float("nan")) == shape
     assert attend(q=None) == attend(starts=None) == attend(rows=-1) == shape
     assert attend(q=8) == align and attend(causal=0, window=3) == unsup and attend(nbytes=100) == small
     assert attend(B=0, q=None) == attend(rows=0, q=None) == 0
-    assert lib.iron_mha_decode_pages_bf16(a, a, a, 4, 16, a, 1, a, 2, 6, 4, 64, -1, 1.0, a, 1 << 40, a, None) == shape
+    assert lib.iron_mha_decode_pages_bf16(a, a, a, 4, 16, a, 1, a, 2, 6, 4, 64, -1, 1.0, a, 1 << 40, a, None, None) == shape
     assert lib.iron_mha_pages_workspace_bytes(96) == 0 and lib.iron_mha_pages_workspace_bytes(64) > 0
 
 
