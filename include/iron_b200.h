@@ -638,10 +638,10 @@ int iron_rope_kv_pages_e4m3(const void* qkv, long long pitch, const void* angles
 
 /* One query a request, q (B, H, D), over its cache: out = softmax(scale * q K^T) V, f32 inside.
  * window >= 0 keeps the keys within `window` positions of the last.  A request of length 0 gets
- * zeros.  `workspace` (iron_mha_pages_workspace_bytes(D) bytes, 16-byte aligned) holds the call's
+ * zeros.  `workspace` (iron_mha_pages_workspace_bytes(D, 0) bytes, 16-byte aligned) holds the call's
  * partial results; it needs no clearing, and two calls that may overlap need one each.  `status`
  * (may be NULL) receives IRON_ERR_TIMEOUT when a bounded wait of the pipeline gives up. */
-long long iron_mha_pages_workspace_bytes(int D);
+long long iron_mha_pages_workspace_bytes(int D, int prompt);
 int iron_mha_decode_pages_bf16(const void* q, const void* pool, const float* scales, int P,
                                int page_size, const int* tables, int width, const int* lengths,
                                int B, int H, int G, int D, int window, float scale,
@@ -652,7 +652,7 @@ int iron_mha_decode_pages_bf16(const void* q, const void* pool, const float* sca
  * at the last positions of its lengths[b] keys.  causal keeps the keys at or before a row's
  * position (window >= 0: and within `window` of it); causal == 0 keeps all of a request's keys
  * (states of another length) and takes no window.  Rows that see nothing are zeros; rows that
- * belong to no request are left as they were. */
+ * belong to no request are left as they were.  workspace: iron_mha_pages_workspace_bytes(D, 1). */
 int iron_mha_prefill_pages_bf16(const void* q, const void* pool, const float* scales, int P,
                                 int page_size, const int* tables, int width, const int* lengths,
                                 const int* row_start, int B, int rows, int H, int G, int D,

@@ -44,26 +44,6 @@ constexpr int kPgStages = 2;                // of a warp's ring; a stage holds k
 constexpr int kPgSegCost = 16;              // units a segment costs beside its own (queries, merge)
 constexpr float kPgLift = 10.f;             // log2 of what probabilities are held times
 
-// A segment that several CTAs share, as the CTA that begins it leaves it for the fold.
-struct PagesRecord {
-  int pieces, row0, head0, col0, cols, pad[3];
-};
-
-struct PagesParams {
-  const __nv_bfloat16* q;
-  const uint8_t* pool;
-  const float* scales;
-  const int* tables;
-  const int* lengths;
-  const int* row_start;     // nullptr: one query a sequence
-  __nv_bfloat16* out;
-  float* partial;
-  PagesRecord* records;
-  int B, H, G, hg, P, width, log_page, causal, window, rows, ctas;   // hg = H / G
-  float scale_log2;
-  int* status;
-};
-
 // A sequence as the kernels see it: its keys, its query rows, and the units a segment spans.
 struct PagesSeq {
   int len, row0, n, unit0;      // keys, first row, rows, first unit any row may see
@@ -103,10 +83,6 @@ struct PgCfg {
   static constexpr int kSmem = kBars + 128 + 1024;
 };
 
-// a / b for a >= 0, b > 0: the 64-bit division is a long routine, and seldom needed
-__device__ __forceinline__ long long div_ll(long long a, int b) {
-  return a >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
-}
 // what a sequence's segments cost in units
 __device__ __forceinline__ long long pages_cost(const PagesParams& p, const PagesSeq& s) {
   return (long long)p.G * s.blocks * (s.units + kPgSegCost);
@@ -134,20 +110,6 @@ __device__ __forceinline__ void mma_f16_16816(float* c, const uint32_t* a, uint3
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// bit 7 of a byte set where the code is NaN (0x7f or 0xff)
-__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
-
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -797,8 +759,9 @@ static int launch_pages_cols(const PagesParams& p, int cols, cudaStream_t stream
 
 using namespace iron;
 
-extern "C" long long iron_mha_pages_workspace_bytes(int D) {
+extern "C" long long iron_mha_pages_workspace_bytes(int D, int prompt) {
   if (D != 64 && D != 128) return 0;
+  if (prompt) return mha_pages_tc_workspace_bytes(D);
   const long long partial = 16ll * D + 32;
   return (long long)kPgCtas * (2 * partial * (long long)sizeof(float) + (long long)sizeof(PagesRecord));
 }
@@ -819,7 +782,7 @@ static int pages_args(PagesParams& p, const void* q, const void* pool, const flo
   if (!aligned16(q) || !aligned16(pool) || !aligned16(out) || !aligned16(workspace) ||
       (reinterpret_cast<uintptr_t>(scales) & 7))
     return IRON_ERR_ALIGN;
-  if (workspace_bytes < iron_mha_pages_workspace_bytes(D)) return IRON_ERR_WORKSPACE;
+  if (workspace_bytes < iron_mha_pages_workspace_bytes(D, row_start != nullptr)) return IRON_ERR_WORKSPACE;
   p.q = (const __nv_bfloat16*)q; p.pool = (const uint8_t*)pool; p.scales = scales; p.tables = tables;
   p.lengths = lengths; p.row_start = row_start; p.out = (__nv_bfloat16*)out; p.records = (PagesRecord*)workspace;
   p.partial = (float*)(p.records + kPgCtas);
@@ -849,7 +812,7 @@ extern "C" int iron_mha_prefill_pages_bf16(const void* q, const void* pool, cons
   const int rc = pages_args(p, q, pool, scales, P, page_size, tables, width, lengths, row_start, B, rows, H, G, D,
                             causal, window, scale, workspace, workspace_bytes, out);
   if (rc) return rc == 1 ? IRON_OK : rc;
-  p.status = status;
   if (!row_start) return IRON_ERR_SHAPE;
-  return D == 64 ? launch_pages<64, 2>(p, (cudaStream_t)stream) : launch_pages<128, 2>(p, (cudaStream_t)stream);
+  p.status = status;
+  return mha_pages_tc(p, D, workspace, (cudaStream_t)stream);
 }

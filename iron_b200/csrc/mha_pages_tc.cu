@@ -1,0 +1,759 @@
+// Attention of ragged query rows over a key/value cache in pages of e4m3 codes, on tcgen05.
+//
+// A work item is a sequence, a KV head and up to 256 query columns -- (row, head of the group)
+// pairs, so grouped heads fill the 128-row MMAs and share what is read -- against the keys any of
+// them sees, in tiles of 128.  One persistent CTA an SM:
+//   warps 8..11   bring the codes: a tile's keys and values go from global memory (page by page,
+//                 the next tile's loads in flight) through registers, where codes become
+//                 halves exactly, into the swizzled shared-memory operands
+//   warps 12, 13  issue S = Q K^T and O += P V for the first and the second 128 columns, each on
+//                 its own so that neither waits for the other's softmax
+//   warps 0..3,   softmax of the first and the second 128 columns: a thread owns a column (one
+//         4..7    lane of tensor memory); scores are read twice, once for the maximum and once for the
+//                 exponentials, and P takes the scores' place in tensor memory as the second
+//                 product's A operand
+// O stays in tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8
+// over the one in use, which after the first tiles is seldom.
+//
+// What the arithmetic is (scales, halves, weights) is the decode kernel's: Q as halves under a
+// power of two a row, a page's key scale on its scores, the logarithm of its value scale added
+// to them; P = p * value scale over the running maximum, in half, held times 2^6 so that with
+// the 2^8 of slack it stays below half's 65504; weights down to 2^-20 of the maximum in use keep full
+// precision.  Maxima, sums and outputs are f32.
+//
+// Items are dealt out by the tile: the tiles of all items, end to end, are cut into equal runs,
+// one a CTA; an item that a boundary cuts leaves partials in the workspace, and a second small
+// launch folds them in order.  Exponentials (16 a clock and SM) and MMAs both need 1024 clocks for
+// 128 columns x 128 keys at D 128.
+//
+// Every mbarrier wait is bounded; a wait that gives up sets the abort flag, every role unwinds,
+// tensor memory is freed and the status word receives IRON_ERR_TIMEOUT.
+#include "common.cuh"
+#include "pages.cuh"
+#include "tc.cuh"
+
+namespace iron {
+
+constexpr int kPtThreads = 448;
+constexpr int kPtRows = 256;          // query columns of an item: two 128-row products
+constexpr int kPtKeys = 128;          // keys of a tile
+constexpr int kPtSub = 16384;         // a 128-row x 128-byte swizzled sub-tile
+constexpr int kPtItemCost = 4;        // what an item costs beside its tiles (a 128-column tile costs 1, two of them 2)
+constexpr int kPtMinShare = 16;
+constexpr float kPtLift = 6.f;        // log2 of what weights are held times
+constexpr float kPtSlack = 8.f;       // log2 of how far the maximum in use may lag
+constexpr int kPtFoldWarps = 8;
+
+template <int D>
+struct PtCfg {
+  static constexpr int kChunks = D / 64;
+  static constexpr int kTile = kChunks * kPtSub;
+  static constexpr int kStages = D == 128 ? 2 : 3;
+  static constexpr int kQ = 0;
+  static constexpr int kK = kQ + 2 * kTile;
+  static constexpr int kV = kK + kStages * kTile;
+  static constexpr int kScale = kV + kStages * kTile;      // [8 warps][2][8] float4
+  static constexpr int kBars = kScale + 8 * 2 * 8 * 16;
+  static constexpr int kSmem = kBars + 256 + 1024;
+  static constexpr int kColS = 0;                          // 2 x 128 columns (P: the first 64 of each)
+  static constexpr int kColO = 256;                        // 2 x D columns
+  static constexpr int kPartial = kPtRows * (D + 2);       // floats: outputs, maxima, sums
+};
+
+struct PtSeq {
+  int len, row0, n, blocks;
+};
+__device__ __forceinline__ PtSeq pt_seq(const PagesParams& p, int b) {
+  PtSeq s;
+  s.len = max(0, (int)min((long long)p.lengths[b], (long long)p.width << p.log_page));
+  s.row0 = min(max(p.row_start[b], 0), p.rows);
+  s.n = max(0, min(p.row_start[b + 1], p.rows) - s.row0);
+  s.blocks = (s.n * p.hg + kPtRows - 1) / kPtRows;
+  return s;
+}
+
+// An item: the columns, the keys that any and that every column sees, the tiles.
+struct PtItem {
+  int b, gh, col0, cols;
+  int len, row0, past;               // of the sequence; past: position of its first row
+  int any_lo, any_hi, all_lo, all_hi;
+  int tile0, tiles;                  // first tile, and how many (at least one: somebody writes the zeros)
+  int t_lo, t_hi;                    // this CTA's piece of them
+  long long at;                      // where the item begins in the dealt-out cost
+};
+__device__ __forceinline__ void pt_block(const PagesParams& p, const PtSeq& s, int j, PtItem& x) {
+  x.col0 = j * kPtRows;
+  x.cols = min(kPtRows, s.n * p.hg - x.col0);
+  x.len = s.len; x.row0 = s.row0; x.past = s.len - s.n;
+  const int first = x.past + x.col0 / p.hg, last = x.past + (x.col0 + x.cols - 1) / p.hg;
+  x.any_lo = p.window >= 0 ? max(0, first - p.window) : 0;
+  x.all_lo = p.window >= 0 ? last - p.window : 0;
+  x.any_hi = p.causal ? max(0, min(s.len, last + 1)) : s.len;
+  x.all_hi = p.causal ? min(s.len, first + 1) : s.len;
+  x.tile0 = x.any_lo / kPtKeys;
+  x.tiles = max(1, (x.any_hi + kPtKeys - 1) / kPtKeys - x.tile0);
+}
+__device__ __forceinline__ int pt_cost(const PtItem& x) { return kPtItemCost + x.tiles * (x.cols > 128 ? 2 : 1); }
+
+__device__ __forceinline__ long long warp_sum_ll(long long v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// The items of [at, end) of the dealt-out cost, in order.
+struct PtWalk {
+  int b, g, j;
+  long long at, end;       // where item (b, g, j) begins; the share's end
+  long long begin;
+  PtSeq seq;
+  __device__ __forceinline__ bool next(const PagesParams& p, PtItem& x) {
+    while (at < end) {
+      while (j >= seq.blocks) {
+        j = 0;
+        if (seq.blocks == 0 || ++g >= p.G) {
+          g = 0;
+          seq = pt_seq(p, ++b);
+        }
+      }
+      pt_block(p, seq, j, x);
+      x.b = b; x.gh = g; x.at = at;
+      const int cost = pt_cost(x), w = x.cols > 128 ? 2 : 1;
+      // a tile belongs to the CTA whose share its cost begins in
+      const long long lo = begin - at - kPtItemCost, hi = end - at - kPtItemCost;
+      x.t_lo = (int)max(0ll, min((long long)x.tiles, (lo + w - 1) / w));
+      x.t_hi = (int)max(0ll, min((long long)x.tiles, (hi + w - 1) / w));
+      at += cost;
+      ++j;
+      if (x.t_lo < x.t_hi) return true;
+    }
+    return false;
+  }
+};
+
+__device__ __forceinline__ uint4 pt_lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// The second product: A in tensor memory (row = lane, two halves of K per 32-bit column).
+__device__ __forceinline__ void tcgen05_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// kind::f16 instruction descriptor: half x half -> f32, M 128, A K-major.
+__host__ __device__ constexpr uint32_t pt_idesc(int n, bool b_n_major) {
+  return (1u << 4) | ((b_n_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+// A row's factor times a page's key scale; never zero, or a masked score, -inf, would become NaN.
+__device__ __forceinline__ float score_factor(float row, uint32_t key_scale) {
+  return fmaxf(row * __uint_as_float(key_scale), 1.17549435e-38f);
+}
+// Sixteen codes -> sixteen halves.
+__device__ __forceinline__ void halves16(const uint4& c, uint4& lo, uint4& hi) {
+  lo = make_uint4(e4m3x2_to_half2(c.x), e4m3x2_to_half2(c.x >> 16), e4m3x2_to_half2(c.y), e4m3x2_to_half2(c.y >> 16));
+  hi = make_uint4(e4m3x2_to_half2(c.z), e4m3x2_to_half2(c.z >> 16), e4m3x2_to_half2(c.w), e4m3x2_to_half2(c.w >> 16));
+}
+
+template <int D>
+__global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const PagesParams p) {
+  using Cfg = PtCfg<D>;
+  extern __shared__ uint8_t pt_smem_raw[];
+  __shared__ long long s_sum[kPtThreads / 32];
+  __shared__ int s_b, s_g, s_j, s_nan;
+  __shared__ long long s_at;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pt_smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kBars);
+  uint64_t* k_full = bars;                          // [kStages]
+  uint64_t* k_empty = k_full + Cfg::kStages;
+  uint64_t* v_full = k_empty + Cfg::kStages;
+  uint64_t* v_empty = v_full + Cfg::kStages;
+  uint64_t* q_full = v_empty + Cfg::kStages;        // [2] each: one a half of the columns
+  uint64_t* s_full = q_full + 2;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_full = p_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  constexpr int kWarps = kPtThreads / 32;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  pdl_launch();
+  pdl_wait();
+  // ---- where this CTA's share begins: a warp sums a stretch of the sequences, a lane their blocks ----
+  const int per_warp = (p.B + kWarps - 1) / kWarps;
+  const int sb = min(warp * per_warp, p.B), se = min(sb + per_warp, p.B);
+  long long mine = 0;
+  for (int b = sb; b < se; ++b) {
+    const PtSeq s = pt_seq(p, b);
+    for (int j = lane; j < s.blocks; j += 32) {
+      PtItem x;
+      pt_block(p, s, j, x);
+      mine += pt_cost(x);
+    }
+  }
+  mine = warp_sum_ll(mine) * p.G;
+  if (lane == 0) s_sum[warp] = mine;
+  if (tid == 0) { s_nan = 0; p.records[blockIdx.x].pieces = 0; }
+  __syncthreads();
+  long long before = 0, total = 0;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += s_sum[w];
+    total += s_sum[w];
+  }
+  const long long share = max((long long)kPtMinShare, div_ll(total + gridDim.x - 1, gridDim.x));
+  const long long begin = (long long)blockIdx.x * share, end = min(begin + share, total);
+  if (begin >= end) return;
+  if (begin >= before && begin < before + mine) {
+    long long acc = before;
+    for (int b = sb; b < se; ++b) {
+      const PtSeq s = pt_seq(p, b);
+      long long one = 0;
+      for (int j = lane; j < s.blocks; j += 32) {
+        PtItem x;
+        pt_block(p, s, j, x);
+        one += pt_cost(x);
+      }
+      one = warp_sum_ll(one);
+      if (begin >= acc + one * p.G) { acc += one * p.G; continue; }
+      const int g = (int)((begin - acc) / one);
+      acc += one * g;
+      for (int j0 = 0; j0 < s.blocks; j0 += 32) {
+        PtItem x;
+        int cost = 0;
+        if (j0 + lane < s.blocks) { pt_block(p, s, j0 + lane, x); cost = pt_cost(x); }
+        long long upto = cost;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long y = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += y;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, cost > 0 && begin < acc + upto);
+        if (hit) {
+          if (lane == __ffs(hit) - 1) { s_b = b; s_g = g; s_j = j0 + lane; s_at = acc + upto - cost; }
+          break;
+        }
+        acc += __shfl_sync(0xffffffffu, upto, 31);
+      }
+      break;
+    }
+  }
+  if (tid == 0) {
+    for (int s = 0; s < Cfg::kStages; ++s) {
+      mbar_init(k_full + s, 128); mbar_init(k_empty + s, 2); mbar_init(v_full + s, 128); mbar_init(v_empty + s, 2);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full + i, 128); mbar_init(s_full + i, 1); mbar_init(p_full + i, 128); mbar_init(o_full + i, 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  PtWalk walk;
+  walk.b = s_b; walk.g = s_g; walk.j = s_j; walk.at = s_at; walk.begin = begin; walk.end = end;
+  walk.seq = pt_seq(p, walk.b);
+  PtItem it;
+  bool ok = true;
+
+  if (warp >= 12) {
+    // ---------------- MMA issuers ----------------
+    if (lane == 0) {
+      const int i = warp - 12;
+      constexpr uint32_t idesc_s = pt_idesc(kPtKeys, false), idesc_o = pt_idesc(D, true);
+      const uint64_t q_desc = make_desc(smem_u32(smem + Cfg::kQ + i * Cfg::kTile), 16, 1024);
+      const uint64_t k_desc0 = make_desc(smem_u32(smem + Cfg::kK), 16, 1024);
+      const uint64_t v_desc0 = make_desc(smem_u32(smem + Cfg::kV), kPtSub, 1024);
+      const uint32_t s_col = tmem + Cfg::kColS + i * 128, o_col = tmem + Cfg::kColO + i * D;
+      int ks = 0, vs = 0, n_item = 0, t = 0;       // t: tiles of this half so far
+      uint32_t kp = 0, vp = 0;
+      auto next_k = [&]() { if (++ks == Cfg::kStages) { ks = 0; kp ^= 1; } };
+      auto next_v = [&]() { if (++vs == Cfg::kStages) { vs = 0; vp ^= 1; } };
+      auto issue_s = [&]() {
+        if (!mbar_wait(k_full + ks, kp, abort_flag)) return false;
+        tcgen05_fence_after();
+        const uint64_t k_desc = k_desc0 + (uint64_t)((ks * Cfg::kTile) >> 4);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t off = (uint64_t)((k >> 2) * (kPtSub >> 4) + (k & 3) * 2);
+          tcgen05_mma_bf16(s_col, q_desc + off, k_desc + off, idesc_s, k != 0);
+        }
+        tcgen05_commit(k_empty + ks);
+        tcgen05_commit(s_full + i);
+        next_k();
+        return true;
+      };
+      while (ok && walk.next(p, it)) {
+        const int n = it.t_hi - it.t_lo;
+        if (it.cols <= i * 128) {
+          // nothing for this half: the tiles are the other's alone
+          for (int u = 0; u < n && ok; ++u) {
+            ok = mbar_wait(k_full + ks, kp, abort_flag) && mbar_wait(v_full + vs, vp, abort_flag);
+            if (!ok) break;
+            mbar_arrive(k_empty + ks);
+            mbar_arrive(v_empty + vs);
+            next_k(); next_v();
+          }
+          continue;
+        }
+        // the softmax's threads have written Q and read the last item's scores and outputs
+        ok = mbar_wait(q_full + i, n_item++ & 1, abort_flag) && issue_s();
+        for (int u = 0; u < n && ok; ++u, ++t) {
+          ok = mbar_wait(v_full + vs, vp, abort_flag) && mbar_wait(p_full + i, t & 1, abort_flag);
+          if (!ok) break;
+          tcgen05_fence_after();
+          const uint64_t v_desc = v_desc0 + (uint64_t)((vs * Cfg::kTile) >> 4);
+#pragma unroll
+          for (int k = 0; k < kPtKeys / 16; ++k)
+            tcgen05_mma_ts(o_col, s_col + k * 8, v_desc + (uint64_t)((k * 16 * 128) >> 4), idesc_o, u > 0 || k != 0);
+          tcgen05_commit(v_empty + vs);
+          tcgen05_commit(o_full + i);
+          next_v();
+          if (u + 1 < n) {
+            // the next scores take P's place: the product that reads it must be done
+            ok = mbar_wait(o_full + i, t & 1, abort_flag) && issue_s();
+          }
+        }
+      }
+    }
+  } else if (warp >= 8) {
+    // ---------------- converters ----------------
+    // A thread has a 16-code piece of eight rows: rows 32 w + 4 r + lane / 8, so a load instruction
+    // takes whole 64- or 128-byte rows.  (With 64 codes a row, four pieces: rows 32 w + 8 r + lane / 4.)
+    constexpr int kPieces = D / 16, kRowsAtOnce = 32 / kPieces, kReps = 32 / kRowsAtOnce;
+    const int w = warp - 8, piece = lane % kPieces, sub_row = lane / kPieces;
+    struct Tile { int key0, any_lo, any_hi, gh, entry; bool partial; };
+    Tile ahead;                    // the tile whose page ids are being looked up
+    int t_at = 0;
+    bool have_item = false;
+    auto advance = [&](Tile& x) {  // the next tile of the share; false at its end
+      while (!have_item || t_at >= it.t_hi) {
+        if (!walk.next(p, it)) return false;
+        have_item = true;
+        t_at = it.t_lo;
+      }
+      x.key0 = (it.tile0 + t_at) * kPtKeys;
+      x.any_lo = it.any_lo; x.any_hi = it.any_hi; x.gh = it.gh;
+      x.partial = x.key0 < it.all_lo || x.key0 + kPtKeys > it.all_hi;
+      const int key = x.key0 + 32 * w + 16 * (lane & 1);      // even lanes: the warp's first page piece
+      int e = -1;
+      if (key < it.any_hi) e = p.tables[(long long)it.b * p.width + (key >> p.log_page)];
+      x.entry = e >= 0 && e < p.P ? e : -1;
+      ++t_at;
+      return true;
+    };
+    uint4 kr[kReps], vr[kReps];
+    const int page_mask = (1 << p.log_page) - 1;
+    auto base_of = [&](const Tile& x, int half, bool& there) {
+      const int e = __shfl_sync(0xffffffffu, x.entry, half);
+      there = e >= 0;
+      const int off = (x.key0 + 32 * w + 16 * half) & page_mask;
+      return p.pool + (((((long long)(there ? e : 0) * p.G + x.gh) * 2) << p.log_page) + off) * D;
+    };
+    auto load = [&](const Tile& x, bool values, uint4* r) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        bool there;
+        const uint8_t* base = base_of(x, half, there) + (values ? ((long long)D << p.log_page) : 0);
+#pragma unroll
+        for (int k = 0; k < kReps / 2; ++k)
+          r[half * (kReps / 2) + k] = there ? ld_stream(base + (k * kRowsAtOnce + sub_row) * D + piece * 16) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto store = [&](uint8_t* tile, int k, const uint4& c) {
+      const int row = 32 * w + k * kRowsAtOnce + sub_row, chunk = 2 * (piece & 3);
+      uint8_t* dst = tile + (piece >> 2) * kPtSub + row * 128;
+      uint4 lo, hi;
+      halves16(c, lo, hi);
+      // the second sub-tile's lanes store their halves in the other order: no two lanes of a phase on one bank
+      const bool swap = D == 128 && (piece >> 2);
+      *reinterpret_cast<uint4*>(dst + (((chunk + (swap ? 1 : 0)) ^ (row & 7)) << 4)) = swap ? hi : lo;
+      *reinterpret_cast<uint4*>(dst + (((chunk + (swap ? 0 : 1)) ^ (row & 7)) << 4)) = swap ? lo : hi;
+    };
+    Tile now, nxt;
+    bool have = advance(now), more = false;
+    if (have) {
+      load(now, false, kr);
+      load(now, true, vr);
+      more = advance(nxt);
+    }
+    int s = 0;
+    uint32_t ph = 0;
+    while (have && ok) {
+      Tile after = nxt;
+      bool more_after = false;
+      ok = mbar_wait_relaxed(k_empty + s, ph ^ 1, abort_flag, 64);
+      if (!ok) break;
+      uint8_t* kt = smem + Cfg::kK + s * Cfg::kTile;
+#pragma unroll
+      for (int k = 0; k < kReps; ++k) store(kt, k, kr[k]);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(k_full + s);
+      if (more) {
+        load(nxt, false, kr);
+        more_after = advance(after);     // page ids of the tile after that
+      }
+      ok = mbar_wait_relaxed(v_empty + s, ph ^ 1, abort_flag, 64);
+      if (!ok) break;
+      uint8_t* vt = smem + Cfg::kV + s * Cfg::kTile;
+      if (now.partial) {
+        // values that no column sees count as zero; a NaN that some see is zero here and comes
+        // back where it is seen when the outputs are written
+#pragma unroll
+        for (int k = 0; k < kReps; ++k) {
+          const int key = now.key0 + 32 * w + k * kRowsAtOnce + sub_row;
+          uint32_t* c = reinterpret_cast<uint32_t*>(&vr[k]);
+          if (key < now.any_lo || key >= now.any_hi) vr[k] = make_uint4(0, 0, 0, 0);
+          if (nan_codes(c[0]) | nan_codes(c[1]) | nan_codes(c[2]) | nan_codes(c[3])) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) c[q] &= ~((nan_codes(c[q]) >> 7) * 0xffu);
+            *reinterpret_cast<volatile int*>(&s_nan) = 1;
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kReps; ++k) store(vt, k, vr[k]);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(v_full + s);
+      if (more) load(nxt, true, vr);
+      if (++s == Cfg::kStages) { s = 0; ph ^= 1; }
+      now = nxt; nxt = after;
+      have = more; more = more_after;
+    }
+  } else {
+    // ---------------- softmax and output ----------------
+    const int i = warp >> 2;                      // which 128 columns
+    const int r = (warp & 3) * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t s_col = lanes + Cfg::kColS + i * 128, o_col = lanes + Cfg::kColO + i * D;
+    float4* scale_at = reinterpret_cast<float4*>(smem + Cfg::kScale) + warp * 16;
+    uint8_t* q_row = smem + Cfg::kQ + i * Cfg::kTile + r * 128;
+    int t = 0;                                    // tiles of this half so far
+    while (ok && walk.next(p, it)) {
+      if (it.cols <= i * 128) continue;
+      const int c = it.col0 + i * 128 + r;        // column of the sequence and KV head
+      const bool live = i * 128 + r < it.cols;
+      const int row = c / p.hg, h = c - row * p.hg, pos = it.past + row;
+      const int hi_key = live ? (p.causal ? min(it.len, pos + 1) : it.len) : 0;
+      const int lo_key = p.window >= 0 ? pos - p.window : 0;
+      const long long out_at = ((long long)(it.row0 + row) * p.H + it.gh * p.hg + h) * D;
+      // ---- Q: halves under a power of two that puts the row's largest in [2^14, 2^15) ----
+      float factor;
+      {
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + out_at);
+        uint4 raw[D / 8];
+#pragma unroll
+        for (int k = 0; k < D / 8; ++k) raw[k] = live ? ld_cached(src + k) : make_uint4(0, 0, 0, 0);
+        float mx = 0.f;
+#pragma unroll
+        for (int k = 0; k < D / 8; ++k) {
+          float f[8];
+          unpack8(raw[k], f);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) mx = fmaxf(mx, fabsf(f[q]));
+        }
+        const int e = min(max((int)(__float_as_uint(mx) >> 23), 15), 254);
+        const float up = __uint_as_float((uint32_t)(268 - e) << 23);
+        factor = p.scale_log2 / up;
+#pragma unroll
+        for (int k = 0; k < D / 8; ++k) {
+          float f[8];
+          unpack8(raw[k], f);
+          *reinterpret_cast<uint4*>(q_row + (k >> 3) * kPtSub + (((k & 7) ^ (r & 7)) << 4)) =
+              make_uint4(pack_half2(f[0] * up, f[1] * up), pack_half2(f[2] * up, f[3] * up),
+                         pack_half2(f[4] * up, f[5] * up), pack_half2(f[6] * up, f[7] * up));
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        tcgen05_fence_before();      // the last item's scores and outputs have been read
+        mbar_arrive(q_full + i);
+      }
+      // ---- scales: lanes 0 .. 7 have a 16-key unit each, ids two tiles ahead, scales one ----
+      const int* table = p.tables + (long long)it.b * p.width;
+      auto entry_of = [&](int tile) {
+        const int key = (it.tile0 + tile) * kPtKeys + 16 * (lane & 7);
+        int e = -1;
+        if (tile < it.t_hi && key < it.any_hi) e = table[key >> p.log_page];
+        return e >= 0 && e < p.P ? e : -1;
+      };
+      auto scale_of = [&](int e) {
+        return e >= 0 ? *reinterpret_cast<const float2*>(p.scales + ((long long)e * p.G + it.gh) * 2) : make_float2(1.f, 0.f);
+      };
+      int e1 = entry_of(it.t_lo);
+      float2 sc = scale_of(e1);
+      e1 = entry_of(it.t_lo + 1);
+      float m_used = -INFINITY, l = 0.f;
+
+      for (int u = it.t_lo; u < it.t_hi && ok; ++u, ++t) {
+        if (lane < 8) {
+          // an absent page: its scores are -inf through the logarithm, its share of the sum nothing
+          scale_at[(u & 1) * 8 + lane] = make_float4(sc.x, __log2f(sc.y), sc.y > 0.f ? 1.f / sc.y : 0.f, 0.f);
+        }
+        __syncwarp();
+        sc = scale_of(e1);
+        e1 = entry_of(u + 2);
+        const uint32_t sc_at = smem_u32(scale_at + (u & 1) * 8);
+        const int key0 = (it.tile0 + u) * kPtKeys;
+        const bool partial = key0 < it.all_lo || key0 + kPtKeys > it.all_hi;
+        ok = mbar_wait(s_full + i, t & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tcgen05_fence_after();
+        auto mask = [&](uint32_t* v, int first) {     // scores of keys first .. first + 31 this column does not see
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if (first + k >= hi_key || first + k < lo_key) v[k] = 0xff800000u;
+        };
+        // ---- the maximum ----
+        float mx = -INFINITY;
+        uint32_t v[2][32];
+        tmem_ld32(s_col, v[0]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          tmem_ld_wait();
+          if (q < 3) tmem_ld32(s_col + (q + 1) * 32, v[(q + 1) & 1]);
+          uint32_t* x = v[q & 1];
+          if (partial) mask(x, key0 + q * 32);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) top = fmaxf(top, __uint_as_float(x[half * 16 + k]));
+            const uint4 f = pt_lds128(sc_at + (q * 2 + half) * 16);
+            mx = fmaxf(mx, fmaf(top, score_factor(factor, f.x), __uint_as_float(f.y)));
+          }
+        }
+        if (__any_sync(0xffffffffu, mx > m_used + kPtSlack)) {
+          const float m_new = fmaxf(m_used, mx);
+          const float corr = m_new == -INFINITY ? 1.f : ex2(m_used - m_new);
+          m_used = m_new;
+          l *= corr;
+          if (u > it.t_lo) {
+            // the scores of this tile came after the last tile's product: the outputs lie still
+#pragma unroll
+            for (int q = 0; q < D / 32; ++q) {
+              tmem_ld32(o_col + q * 32, v[0]);
+              tmem_ld_wait();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) v[0][k] = __float_as_uint(__uint_as_float(v[0][k]) * corr);
+              tmem_st16(o_col + q * 32, v[0]);
+              tmem_st16(o_col + q * 32 + 16, v[0] + 16);
+            }
+          }
+        }
+        // ---- weights: P over the scores' place, and their sum ----
+        const float base = (m_used == -INFINITY ? 0.f : m_used) - kPtLift;
+        tmem_ld32(s_col, v[0]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          tmem_ld_wait();
+          if (q < 3) tmem_ld32(s_col + (q + 1) * 32, v[(q + 1) & 1]);
+          uint32_t* x = v[q & 1];
+          if (partial) mask(x, key0 + q * 32);
+          uint32_t out[16];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint4 f = pt_lds128(sc_at + (q * 2 + half) * 16);
+            const float a = score_factor(factor, f.x), b = __uint_as_float(f.y) - base;
+            float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+            for (int k = 0; k < 16; k += 2) {
+              const float p0 = ex2(fmaf(__uint_as_float(x[half * 16 + k]), a, b));
+              const float p1 = ex2(fmaf(__uint_as_float(x[half * 16 + k + 1]), a, b));
+              sum0 += p0; sum1 += p1;
+              out[half * 8 + k / 2] = pack_half2(p0, p1);
+            }
+            l = fmaf(sum0 + sum1, __uint_as_float(f.z), l);
+          }
+          // columns 16 q .. of P lie on scores that have been read: 16 q + 16 <= 32 (q + 1)
+          if (q < 3) tmem_ld_wait();
+          tmem_st16(s_col + q * 16, out);
+        }
+        tmem_st_wait();
+        tcgen05_fence_before();
+        mbar_arrive(p_full + i);
+      }
+      // ---- the item's results ----
+      if (ok) ok = mbar_wait(o_full + i, (t - 1) & 1, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tcgen05_fence_after();
+      const bool direct = it.t_lo == 0 && it.t_hi == it.tiles;
+      float* part = p.partial + ((long long)blockIdx.x * 2 + (it.t_lo == 0 ? 1 : 0)) * Cfg::kPartial;
+      const bool nans = *reinterpret_cast<volatile int*>(&s_nan) != 0;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+      for (int q = 0; q < D / 32; ++q) {
+        uint32_t v[32];
+        __syncwarp();
+        tmem_ld32(o_col + q * 32, v);
+        tmem_ld_wait();
+        if (nans && live) {
+          // NaN codes of partial tiles were taken as zero: they are NaN to the rows that see them
+          uint32_t hit = 0;
+          const int from = max(lo_key, (it.tile0 + it.t_lo) * kPtKeys), to = min(hi_key, (it.tile0 + it.t_hi) * kPtKeys);
+          for (int key = max(from, 0); key < to; ++key) {
+            const int k0 = key / kPtKeys * kPtKeys;
+            if (k0 >= it.all_lo && k0 + kPtKeys <= it.all_hi) { key = k0 + kPtKeys - 1; continue; }
+            const int e = table[key >> p.log_page];
+            if (e < 0 || e >= p.P) continue;
+            const long long block = ((long long)e * p.G + it.gh) * 2 + 1;
+            const uint32_t* code = reinterpret_cast<const uint32_t*>(
+                p.pool + ((block << p.log_page) + (key & ((1 << p.log_page) - 1))) * D + q * 32);
+            for (int k = 0; k < 8; ++k) {
+              const uint32_t b = nan_codes(code[k]) >> 7;
+              hit |= ((b & 1) | (b >> 7 & 2) | (b >> 14 & 4) | (b >> 21 & 8)) << (4 * k);
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if (hit >> k & 1) v[k] = 0x7fc00000u;
+        }
+        if (live && direct) {
+          uint32_t o[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            o[k] = l == 0.f ? 0u : pack_bf16x2(__uint_as_float(v[2 * k]) * inv, __uint_as_float(v[2 * k + 1]) * inv);
+#pragma unroll
+          for (int k = 0; k < 16; k += 4)
+            *reinterpret_cast<uint4*>(p.out + out_at + q * 32 + 2 * k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+        } else if (live) {
+#pragma unroll
+          for (int k = 0; k < 32; k += 4)
+            *reinterpret_cast<uint4*>(part + (i * 128 + r) * D + q * 32 + k) = make_uint4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+        }
+      }
+      if (!direct) {
+        if (live) {
+          part[kPtRows * D + i * 128 + r] = m_used;
+          part[kPtRows * D + kPtRows + i * 128 + r] = l;
+        }
+        if (tid == 0 && it.t_lo == 0) {
+          const int w = it.cols > 128 ? 2 : 1;
+          PagesRecord rec;
+          rec.pieces = (int)((it.at + kPtItemCost + (long long)(it.tiles - 1) * w) / share) - (int)blockIdx.x + 1;
+          rec.row0 = it.row0; rec.head0 = it.gh * p.hg; rec.col0 = it.col0;
+          rec.cols = it.cols;
+          p.records[blockIdx.x] = rec;
+        }
+      }
+    }
+  }
+
+  if (!ok) {
+    // a wait gave up: give what is in flight a millisecond, many times what it takes
+    const unsigned long long t0 = global_ns();
+    while (global_ns() - t0 < 1000000ull) {}
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if (tid == 0 && *abort_flag && p.status) *p.status = IRON_ERR_TIMEOUT;
+  if (warp == 12) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+// Folds the partials of an item that several CTAs share, in the order of its keys: one CTA for
+// eight columns of each main CTA's record, a warp a column, a lane a stretch of d.
+template <int D>
+__global__ void __launch_bounds__(kPtFoldWarps * 32) mha_pages_tc_fold_kernel(const PagesParams p) {
+  using Cfg = PtCfg<D>;
+  constexpr int PER = D / 32, kBatch = 4;
+  pdl_launch();
+  pdl_wait();
+  const PagesRecord r = p.records[blockIdx.x];
+  const int lane = threadIdx.x & 31, c = blockIdx.y * kPtFoldWarps + (threadIdx.x >> 5);
+  if (r.pieces <= 1 || c >= r.cols) return;
+  float m = -INFINITY, l = 0.f, o[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) o[j] = 0.f;
+  for (int i0 = 0; i0 < r.pieces; i0 += kBatch) {
+    float x[kBatch][PER], mi[kBatch], li[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int i = min(i0 + k, r.pieces - 1);   // past the end: loaded again, not counted
+      // the piece that begins the item lies in its CTA's second slot, the others in the first
+      const float* src = p.partial + ((long long)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * Cfg::kPartial;
+      mi[k] = src[kPtRows * D + c];
+      li[k] = src[kPtRows * D + kPtRows + c];
+      const float2* v = reinterpret_cast<const float2*>(src + c * D + lane * PER);
+#pragma unroll
+      for (int j = 0; j < PER / 2; ++j) { const float2 y = v[j]; x[k][2 * j] = y.x; x[k][2 * j + 1] = y.y; }
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (i0 + k >= r.pieces) break;
+      const float m_new = fmaxf(m, mi[k]), safe = m_new == -INFINITY ? 0.f : m_new;
+      const float f = ex2(m - safe), fi = ex2(mi[k] - safe);
+      m = m_new;
+      l = l * f + li[k] * fi;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) o[j] = o[j] * f + x[k][j] * fi;
+    }
+  }
+  const int row = (r.col0 + c) / p.hg, h = (r.col0 + c) - row * p.hg;
+  __nv_bfloat16* dst = p.out + ((long long)(r.row0 + row) * p.H + r.head0 + h) * D + lane * PER;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int j = 0; j < PER; j += 2)
+    *reinterpret_cast<uint32_t*>(dst + j) = l == 0.f ? 0u : pack_bf16x2(o[j] * inv, o[j + 1] * inv);
+}
+
+long long mha_pages_tc_workspace_bytes(int D) {
+  const long long partial = D == 64 ? PtCfg<64>::kPartial : PtCfg<128>::kPartial;
+  return kSMs * ((long long)sizeof(PagesRecord) + 2 * partial * (long long)sizeof(float));
+}
+
+template <int D>
+static int launch_pages_tc(PagesParams p, void* workspace, cudaStream_t stream) {
+  p.records = (PagesRecord*)workspace;
+  p.partial = (float*)(p.records + kSMs);
+  static DeviceOnce configured;
+  if (!configured.done()) {
+    if (cudaFuncSetAttribute(mha_pages_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, PtCfg<D>::kSmem) !=
+        cudaSuccess)
+      return IRON_ERR_LAUNCH;
+    configured.mark();
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kSMs);
+  cfg.blockDim = dim3(kPtThreads);
+  cfg.dynamicSmemBytes = PtCfg<D>::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  fill_pdl_attr(cfg, attr);
+  if (cudaLaunchKernelEx(&cfg, mha_pages_tc_kernel<D>, p) != cudaSuccess) return IRON_ERR_LAUNCH;
+  const long long cols = (long long)p.rows * p.hg;
+  cfg.gridDim = dim3(kSMs, (unsigned)(((cols < kPtRows ? cols : kPtRows) + kPtFoldWarps - 1) / kPtFoldWarps));
+  cfg.blockDim = dim3(kPtFoldWarps * 32);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, mha_pages_tc_fold_kernel<D>, p) == cudaSuccess ? IRON_OK : IRON_ERR_LAUNCH;
+}
+
+int mha_pages_tc(const PagesParams& p, int D, void* workspace, cudaStream_t stream) {
+  return D == 64 ? launch_pages_tc<64>(p, workspace, stream) : launch_pages_tc<128>(p, workspace, stream);
+}
+
+}  // namespace iron

@@ -1,5 +1,5 @@
 // What the kernels of the paged 8-bit key/value cache share: the page sizes taken, the e4m3
-// conversions, and the power-of-two scale of a (page, KV head).
+// conversions, the power-of-two scale of a (page, KV head), and what the attention calls are given.
 #pragma once
 #include "common.cuh"
 
@@ -45,5 +45,47 @@ __device__ __forceinline__ float pow2_scale(float amax) {
   e = max(e, -60);   // zero and subnormal magnitudes end here
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
+
+// A segment that several CTAs share, as the CTA that begins it leaves it for the fold.
+struct PagesRecord {
+  int pieces, row0, head0, col0, cols, pad[3];
+};
+
+struct PagesParams {
+  const __nv_bfloat16* q;
+  const uint8_t* pool;
+  const float* scales;
+  const int* tables;
+  const int* lengths;
+  const int* row_start;     // nullptr: one query a sequence
+  __nv_bfloat16* out;
+  float* partial;
+  PagesRecord* records;
+  int B, H, G, hg, P, width, log_page, causal, window, rows, ctas;   // hg = H / G
+  float scale_log2;
+  int* status;
+};
+
+// a / b for a >= 0, b > 0: the 64-bit division is a long routine, and seldom needed
+__device__ __forceinline__ long long div_ll(long long a, int b) {
+  return a >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// bit 7 of a byte set where the code is NaN (0x7f or 0xff)
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// The ragged form on tcgen05 (mha_pages_tc.cu).
+long long mha_pages_tc_workspace_bytes(int D);
+int mha_pages_tc(const PagesParams& p, int D, void* workspace, cudaStream_t stream);
 
 }  // namespace iron

@@ -572,22 +572,27 @@ def gemm_rows_qkv_rope(X, Wqkv, angles, q_out, k_cache, v_cache, positions, *, H
 E4M3 = torch.float8_e4m3fn
 
 
-def _on_device(*ts) -> None:
-    """Every tensor is a contiguous one of the current CUDA device (launches go to its stream)."""
-    dev = torch.cuda.current_device() if torch.cuda.is_available() else None
+def _on_device(*ts) -> int:
+    """Every tensor is a contiguous one of the current CUDA device; returns that device's current stream.
+
+    These calls are a few microseconds of work on the device, so the checks are kept as cheap."""
+    dev = ts[0].get_device()
     for t in ts:
-        if not t.is_cuda:
-            raise RuntimeError("iron_b200 kernels take CUDA tensors only (no CPU fallback)")
-        if t.get_device() != dev:
+        if t.get_device() != dev or dev < 0 or not t.is_contiguous():
+            if not t.is_cuda:
+                raise RuntimeError("iron_b200 kernels take CUDA tensors only (no CPU fallback)")
+            if not t.is_contiguous():
+                raise ValueError("iron_b200 kernels take contiguous tensors")
             raise ValueError(f"a tensor of cuda:{t.get_device()} in a call on cuda:{dev}")
-        if not t.is_contiguous():
-            raise ValueError("iron_b200 kernels take contiguous tensors")
+    if dev != torch.cuda.current_device():
+        raise ValueError(f"tensors of cuda:{dev} in a call on cuda:{torch.cuda.current_device()}")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _int32(**ts) -> None:
-    for name, t in ts.items():
-        if t.dtype != torch.int32:
-            raise TypeError(f"{name} is int32, not {t.dtype}")
+def _int32(names: str, *ts) -> None:
+    for t in ts:
+        if t.dtype is not torch.int32:
+            raise TypeError(f"{names} are int32, not {t.dtype}")
 
 
 def _pool_sizes(pool, scales):
@@ -619,23 +624,21 @@ def page_step(tables, lengths, new_tokens, pages, ring, *, page_size, rows, leng
     B, width = tables.shape
     if rows < 0:
         raise ValueError(f"rows ({rows}) is negative")
-    device = tables.device
-    new = lambda n: torch.empty(n, dtype=torch.int32, device=device)  # noqa: E731
-    slots = new(rows) if slots is None else slots
-    positions = new(rows) if positions is None else positions
-    row_start = new(B + 1) if row_start is None else row_start
-    lengths_out = new(B) if lengths_out is None else lengths_out
-    ring_out = new(4) if ring_out is None else ring_out
-    if (slots.shape, positions.shape, row_start.shape) != ((rows,), (rows,), (B + 1,)) or \
-            lengths_out.shape != lengths.shape or ring_out.shape != ring.shape:
-        raise ValueError("outputs are slots (rows,), positions (rows,), row_start (B + 1,), lengths_out (B,), ring_out (4,)")
-    _int32(tables=tables, lengths=lengths, new_tokens=new_tokens, pages=pages, ring=ring, slots=slots,
-           positions=positions, row_start=row_start, lengths_out=lengths_out, ring_out=ring_out)
-    _on_device(tables, lengths, new_tokens, pages, ring, slots, positions, row_start, lengths_out, ring_out)
+    outs = (slots, positions, row_start, lengths_out, ring_out)
+    sizes = (rows, rows, B + 1, B, 4)
+    if any(t is None for t in outs):   # one allocation for all that are missing
+        made = torch.empty(2 * B + 2 * rows + 5, dtype=torch.int32, device=tables.device).split(sizes)
+        outs = tuple(m if t is None else t for t, m in zip(outs, made))
+    for t, n in zip(outs, sizes):
+        if t.dim() != 1 or t.shape[0] != n:
+            raise ValueError("outputs are slots (rows,), positions (rows,), row_start (B + 1,), lengths_out (B,), ring_out (4,)")
+    _int32("page_step's tensors", tables, lengths, new_tokens, pages, ring, *outs)
+    stream = _on_device(tables, lengths, new_tokens, pages, ring, *outs)
+    slots, positions, row_start, lengths_out, ring_out = outs
     call("iron_page_step", tables.data_ptr(), width, lengths.data_ptr(), new_tokens.data_ptr(), B, pages.data_ptr(),
          pages.shape[0], ring.data_ptr(), int(page_size), int(rows), lengths_out.data_ptr(), ring_out.data_ptr(),
-         slots.data_ptr(), positions.data_ptr(), row_start.data_ptr(), _stream())
-    return slots, positions, row_start, lengths_out, ring_out
+         slots.data_ptr(), positions.data_ptr(), row_start.data_ptr(), stream)
+    return outs
 
 
 def rope_kv_pages(qkv, angles, q_out, pool, scales, slots, positions, *, H, G, D):
@@ -656,20 +659,28 @@ def rope_kv_pages(qkv, angles, q_out, pool, scales, slots, positions, *, H, G, D
                          f"are not for {rows} rows")
     if angles.dim() != 2 or angles.shape[1] != D:
         raise ValueError(f"angles {tuple(angles.shape)} are not (positions, {D})")
-    _int32(slots=slots, positions=positions)
-    _on_device(qkv[:1], angles, q_out, pool, scales, slots, positions)
+    _int32("slots and positions", slots, positions)
+    dense = rows <= 1 or qkv.stride(0) == qkv.shape[1]
+    stream = _on_device(angles, q_out, pool, scales, slots, positions, qkv if dense else qkv[:1])
     call("iron_rope_kv_pages_e4m3", qkv.data_ptr(), qkv.stride(0) if rows > 1 else qkv.shape[1], angles.data_ptr(),
          q_out.data_ptr(), pool.data_ptr(), scales.data_ptr(), P, page, slots.data_ptr(), positions.data_ptr(), rows,
-         H, G, D, angles.shape[0], _stream())
+         H, G, D, angles.shape[0], stream)
     return q_out
 
 
-def pages_workspace(D: int, device=None) -> torch.Tensor:
-    """The partial results of one attention call over a paged cache; calls that may overlap need one each."""
-    return torch.empty(_lib.load().iron_mha_pages_workspace_bytes(D), dtype=torch.uint8, device=device or "cuda")
+_PAGES_BYTES: dict[tuple, int] = {}
 
 
-def _pages_attention(Q, pool, scales, tables, lengths, out, workspace):
+def pages_workspace(D: int, prompt: bool = False, device=None) -> torch.Tensor:
+    """The partial results of one attention call over a paged cache (``prompt``: of
+    ``mha_prefill_pages``); calls that may overlap need one each."""
+    n = _PAGES_BYTES.get((D, prompt))
+    if n is None:
+        n = _PAGES_BYTES[D, prompt] = _lib.load().iron_mha_pages_workspace_bytes(D, int(prompt))
+    return torch.empty(n, dtype=torch.uint8, device=device or "cuda")
+
+
+def _pages_attention(Q, pool, scales, tables, lengths, out, workspace, row_start=None):
     _bf16(Q, out)
     P, G, page, D = _pool_sizes(pool, scales)
     if Q.dim() != 3 or Q.shape[2] != D or Q.shape[1] % G:
@@ -681,10 +692,10 @@ def _pages_attention(Q, pool, scales, tables, lengths, out, workspace):
     elif out.shape != Q.shape:
         raise ValueError(f"out {tuple(out.shape)} is not {tuple(Q.shape)}")
     if workspace is None:
-        workspace = pages_workspace(D, Q.device)
-    _int32(tables=tables, lengths=lengths)
-    _on_device(Q, out, pool, scales, tables, lengths, workspace)
-    return P, G, page, D, out, workspace
+        workspace = pages_workspace(D, row_start is not None, Q.device)
+    starts = () if row_start is None else (row_start,)
+    _int32("tables, lengths and row_start", tables, lengths, *starts)
+    return P, G, page, D, out, workspace, _on_device(Q, out, pool, scales, tables, lengths, workspace, *starts)
 
 
 def mha_decode_pages(Q, pool, scales, tables, lengths, out=None, *, window=None, scale=None, workspace=None,
@@ -696,11 +707,11 @@ def mha_decode_pages(Q, pool, scales, tables, lengths, out=None, *, window=None,
     that receives ``IRON_ERR_TIMEOUT`` when a bounded wait gives up."""
     if Q.shape[:1] != lengths.shape:
         raise ValueError(f"Q {tuple(Q.shape)} is not one query for each of {tuple(lengths.shape)} requests")
-    P, G, page, D, out, workspace = _pages_attention(Q, pool, scales, tables, lengths, out, workspace)
+    P, G, page, D, out, workspace, stream = _pages_attention(Q, pool, scales, tables, lengths, out, workspace)
     call("iron_mha_decode_pages_bf16", Q.data_ptr(), pool.data_ptr(), scales.data_ptr(), P, page, tables.data_ptr(),
          tables.shape[1], lengths.data_ptr(), Q.shape[0], Q.shape[1], G, D, -1 if window is None else int(window),
          1.0 / math.sqrt(D) if scale is None else float(scale), workspace.data_ptr(), workspace.numel(),
-         out.data_ptr(), _ptr(status), _stream())
+         out.data_ptr(), _ptr(status), stream)
     return out
 
 
@@ -716,13 +727,11 @@ def mha_prefill_pages(Q, pool, scales, tables, lengths, row_start, out=None, *, 
         raise ValueError(f"row_start {tuple(row_start.shape)} is not ({B + 1},)")
     if window is not None and not causal:
         raise ValueError("a window goes with the causal mask")
-    _int32(row_start=row_start)
-    P, G, page, D, out, workspace = _pages_attention(Q, pool, scales, tables, lengths, out, workspace)
-    _on_device(row_start)
+    P, G, page, D, out, workspace, stream = _pages_attention(Q, pool, scales, tables, lengths, out, workspace, row_start)
     call("iron_mha_prefill_pages_bf16", Q.data_ptr(), pool.data_ptr(), scales.data_ptr(), P, page, tables.data_ptr(),
          tables.shape[1], lengths.data_ptr(), row_start.data_ptr(), B, Q.shape[0], Q.shape[1], G, D, int(bool(causal)),
          -1 if window is None else int(window), 1.0 / math.sqrt(D) if scale is None else float(scale),
-         workspace.data_ptr(), workspace.numel(), out.data_ptr(), _ptr(status), _stream())
+         workspace.data_ptr(), workspace.numel(), out.data_ptr(), _ptr(status), stream)
     return out
 
 

@@ -123,7 +123,7 @@ def test_the_c_entries_refuse_before_any_launch():
     assert attend(q=8) == align and attend(causal=0, window=3) == unsup and attend(nbytes=100) == small
     assert attend(B=0, q=None) == attend(rows=0, q=None) == 0
     assert lib.iron_mha_decode_pages_bf16(a, a, a, 4, 16, a, 1, a, 2, 6, 4, 64, -1, 1.0, a, 1 << 40, a, None, None) == shape
-    assert lib.iron_mha_pages_workspace_bytes(96) == 0 and lib.iron_mha_pages_workspace_bytes(64) > 0
+    assert lib.iron_mha_pages_workspace_bytes(96, 0) == 0 < lib.iron_mha_pages_workspace_bytes(64, 0) < lib.iron_mha_pages_workspace_bytes(64, 1)
 
 
 def test_the_plain_step_hands_pages_on_in_order():
