@@ -773,7 +773,7 @@ static int pages_args(PagesParams& p, const void* q, const void* pool, const flo
   const int log_page = log2_page(page_size);
   if (B < 0 || rows < 0 || H <= 0 || G <= 0 || H % G || (D != 64 && D != 128) || P <= 0 || width <= 0 || log_page < 0)
     return IRON_ERR_SHAPE;
-  if (G > 65535 || (long long)P * G > 0x7fffffffll || (long long)P * page_size > 0x7fffffffll || (long long)rows * H > 0x7fffffffll) return IRON_ERR_SHAPE;
+  if (G > 65535 || (long long)P * G * (page_size / 8) > 0x7fffffffll || (long long)P * page_size > 0x7fffffffll || (long long)rows * H > 0x7fffffffll) return IRON_ERR_SHAPE;
   if ((long long)width * page_size > 0x7fffffffll) return IRON_ERR_SHAPE;
   if (window >= 0 && !causal) return IRON_ERR_UNSUPPORTED;
   if (!(scale > 0.f)) return IRON_ERR_SHAPE;

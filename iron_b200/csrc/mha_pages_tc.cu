@@ -3,10 +3,10 @@
 // A work item is a sequence, a KV head and up to 256 query columns -- (row, head of the group)
 // pairs, so grouped heads fill the 128-row MMAs and share what is read -- against the keys any of
 // them sees, in tiles of 128.  One persistent CTA an SM:
-//   warps 8..11   bring the codes: a tile's keys and values go from global memory (page by page,
-//                 the next tile's loads in flight) through registers, where codes become
-//                 halves exactly, into the swizzled shared-memory operands
-//   warps 12, 13  issue S = Q K^T and O += P V for the first and the second 128 columns, each on
+//   warps 8..11,  bring the codes: a tile's keys (8..11) and values (12..15) go from global memory,
+//         12..15  page by page, the next tile's loads in flight, through registers, where codes
+//                 become halves exactly, into the swizzled shared-memory operands
+//   warps 16, 17  issue S = Q K^T and O += P V for the first and the second 128 columns, each on
 //                 its own so that neither waits for the other's softmax
 //   warps 0..3,   softmax of the first and the second 128 columns: a thread owns a column (one
 //         4..7    lane of tensor memory); scores are read twice, once for the maximum and once for the
@@ -34,15 +34,21 @@
 
 namespace iron {
 
-constexpr int kPtThreads = 448;
+constexpr int kPtThreads = 640;
 constexpr int kPtRows = 256;          // query columns of an item: two 128-row products
 constexpr int kPtKeys = 128;          // keys of a tile
 constexpr int kPtSub = 16384;         // a 128-row x 128-byte swizzled sub-tile
-constexpr int kPtItemCost = 4;        // what an item costs beside its tiles (a 128-column tile costs 1, two of them 2)
-constexpr int kPtMinShare = 16;
+// What the tiles of one and of two 128-column halves cost, and an item beside its tiles, as measured:
+// one half alone waits for its own chain of products and exponentials.
+constexpr int kPtCostOne = 4, kPtCostTwo = 6, kPtItemCost = 12;
+constexpr int kPtMinShare = 36;
 constexpr float kPtLift = 6.f;        // log2 of what weights are held times
 constexpr float kPtSlack = 8.f;       // log2 of how far the maximum in use may lag
 constexpr int kPtFoldWarps = 8;
+constexpr int kPtSlots = 4;           // items looked up ahead
+constexpr int kPtScales = 4;          // tiles whose scales are held: the converters are two ahead at most
+constexpr int kPtPitch = 80;          // bytes between the rows a warp turns its outputs in: 16-byte pieces of 8 rows on 8 bank groups
+constexpr int kPtRoles = 18;          // warps that read them
 
 template <int D>
 struct PtCfg {
@@ -52,10 +58,12 @@ struct PtCfg {
   static constexpr int kQ = 0;
   static constexpr int kK = kQ + 2 * kTile;
   static constexpr int kV = kK + kStages * kTile;
-  static constexpr int kScale = kV + kStages * kTile;      // [8 warps][2][8] float4
-  static constexpr int kBars = kScale + 8 * 2 * 8 * 16;
-  static constexpr int kSmem = kBars + 256 + 1024;
-  static constexpr int kColS = 0;                          // 2 x 128 columns (P: the first 64 of each)
+  static constexpr int kScale = kV + kStages * kTile;      // a ring of tiles: [8 units] float4
+  static constexpr int kItems = kScale + kPtScales * 8 * 16;   // a ring of items
+  static constexpr int kOut = kItems + kPtSlots * 64;      // [8 warps] 32 rows x 64 bytes, kPtPitch apart
+  static constexpr int kBars = kOut + 8 * 32 * kPtPitch;
+  static constexpr int kSmem = kBars + 512 + 1024;
+  static constexpr int kColS = 0;                          // 2 x 128 columns (P: the last 64 of each)
   static constexpr int kColO = 256;                        // 2 x D columns
   static constexpr int kPartial = kPtRows * (D + 2);       // floats: outputs, maxima, sums
 };
@@ -73,13 +81,12 @@ __device__ __forceinline__ PtSeq pt_seq(const PagesParams& p, int b) {
 }
 
 // An item: the columns, the keys that any and that every column sees, the tiles.
-struct PtItem {
-  int b, gh, col0, cols;
-  int len, row0, past;               // of the sequence; past: position of its first row
+struct alignas(64) PtItem {
+  int b, gh, col0, cols;             // no columns: the share's end
+  int len, row0, past, whole;        // of the sequence; past: position of its first row; whole: no other CTA has tiles of it
   int any_lo, any_hi, all_lo, all_hi;
   int tile0, tiles;                  // first tile, and how many (at least one: somebody writes the zeros)
   int t_lo, t_hi;                    // this CTA's piece of them
-  long long at;                      // where the item begins in the dealt-out cost
 };
 __device__ __forceinline__ void pt_block(const PagesParams& p, const PtSeq& s, int j, PtItem& x) {
   x.col0 = j * kPtRows;
@@ -93,7 +100,8 @@ __device__ __forceinline__ void pt_block(const PagesParams& p, const PtSeq& s, i
   x.tile0 = x.any_lo / kPtKeys;
   x.tiles = max(1, (x.any_hi + kPtKeys - 1) / kPtKeys - x.tile0);
 }
-__device__ __forceinline__ int pt_cost(const PtItem& x) { return kPtItemCost + x.tiles * (x.cols > 128 ? 2 : 1); }
+__device__ __forceinline__ int pt_tile_cost(const PtItem& x) { return x.cols > 128 ? kPtCostTwo : kPtCostOne; }
+__device__ __forceinline__ int pt_cost(const PtItem& x) { return kPtItemCost + x.tiles * pt_tile_cost(x); }
 
 __device__ __forceinline__ long long warp_sum_ll(long long v) {
 #pragma unroll
@@ -105,7 +113,7 @@ __device__ __forceinline__ long long warp_sum_ll(long long v) {
 struct PtWalk {
   int b, g, j;
   long long at, end;       // where item (b, g, j) begins; the share's end
-  long long begin;
+  long long begin, last_tile;   // last_tile: where the item's last tile begins
   PtSeq seq;
   __device__ __forceinline__ bool next(const PagesParams& p, PtItem& x) {
     while (at < end) {
@@ -117,12 +125,14 @@ struct PtWalk {
         }
       }
       pt_block(p, seq, j, x);
-      x.b = b; x.gh = g; x.at = at;
-      const int cost = pt_cost(x), w = x.cols > 128 ? 2 : 1;
+      x.b = b; x.gh = g;
+      const int cost = pt_cost(x), w = pt_tile_cost(x);
       // a tile belongs to the CTA whose share its cost begins in
       const long long lo = begin - at - kPtItemCost, hi = end - at - kPtItemCost;
       x.t_lo = (int)max(0ll, min((long long)x.tiles, (lo + w - 1) / w));
       x.t_hi = (int)max(0ll, min((long long)x.tiles, (hi + w - 1) / w));
+      x.whole = x.t_lo == 0 && x.t_hi == x.tiles;
+      last_tile = at + kPtItemCost + (long long)(x.tiles - 1) * w;
       at += cost;
       ++j;
       if (x.t_lo < x.t_hi) return true;
@@ -159,6 +169,41 @@ __device__ __forceinline__ void tcgen05_mma_ts(uint32_t d_tmem, uint32_t a_tmem,
 __host__ __device__ constexpr uint32_t pt_idesc(int n, bool b_n_major) {
   return (1u << 4) | ((b_n_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
+// Waits for a tensor-memory load and names its registers, so that no use of them moves above.
+__device__ __forceinline__ void tmem_ld_wait32(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               ::"memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Two f32 fused multiply-adds, and two sums, in one instruction each.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 // A row's factor times a page's key scale; never zero, or a masked score, -inf, would become NaN.
 __device__ __forceinline__ float score_factor(float row, uint32_t key_scale) {
   return fmaxf(row * __uint_as_float(key_scale), 1.17549435e-38f);
@@ -186,8 +231,13 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
   uint64_t* s_full = q_full + 2;
   uint64_t* p_full = s_full + 2;
   uint64_t* o_full = p_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+  uint64_t* o_free = o_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_free + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint64_t* item_full = o_free + 3;                 // [kPtSlots] each (behind the two words above)
+  uint64_t* item_empty = item_full + kPtSlots;
+  uint64_t* scale_full = item_empty + kPtSlots;     // [kPtScales]
+  PtItem* items = reinterpret_cast<PtItem*>(smem + Cfg::kItems);
   constexpr int kWarps = kPtThreads / 32;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -257,11 +307,14 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + i, 128); mbar_init(s_full + i, 1); mbar_init(p_full + i, 128); mbar_init(o_full + i, 1);
+      mbar_init(o_free + i, 128);
     }
+    for (int s = 0; s < kPtSlots; ++s) { mbar_init(item_full + s, 1); mbar_init(item_empty + s, kPtRoles); }
+    for (int s = 0; s < kPtScales; ++s) mbar_init(scale_full + s, 4);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 12) {
+  if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(512)
                  : "memory");
@@ -272,28 +325,72 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
   tcgen05_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  PtWalk walk;
-  walk.b = s_b; walk.g = s_g; walk.j = s_j; walk.at = s_at; walk.begin = begin; walk.end = end;
-  walk.seq = pt_seq(p, walk.b);
-  PtItem it;
   bool ok = true;
+  // The next item, from the ring that warp 18 fills; `take` copies what the role needs of it.
+  int slot = 0;
+  uint32_t slot_phase = 0;
+  auto next_item = [&](auto&& take) {
+    ok = ok && mbar_wait(item_full + slot, slot_phase, abort_flag);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) return false;
+    const PtItem& x = items[slot];
+    const bool more = x.cols > 0;
+    if (more) take(x);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(item_empty + slot);
+    if (++slot == kPtSlots) { slot = 0; slot_phase ^= 1; }
+    return more;
+  };
 
-  if (warp >= 12) {
-    // ---------------- MMA issuers ----------------
-    if (lane == 0) {
-      const int i = warp - 12;
-      constexpr uint32_t idesc_s = pt_idesc(kPtKeys, false), idesc_o = pt_idesc(D, true);
-      const uint64_t q_desc = make_desc(smem_u32(smem + Cfg::kQ + i * Cfg::kTile), 16, 1024);
-      const uint64_t k_desc0 = make_desc(smem_u32(smem + Cfg::kK), 16, 1024);
-      const uint64_t v_desc0 = make_desc(smem_u32(smem + Cfg::kV), kPtSub, 1024);
-      const uint32_t s_col = tmem + Cfg::kColS + i * 128, o_col = tmem + Cfg::kColO + i * D;
-      int ks = 0, vs = 0, n_item = 0, t = 0;       // t: tiles of this half so far
-      uint32_t kp = 0, vp = 0;
-      auto next_k = [&]() { if (++ks == Cfg::kStages) { ks = 0; kp ^= 1; } };
-      auto next_v = [&]() { if (++vs == Cfg::kStages) { vs = 0; vp ^= 1; } };
-      auto issue_s = [&]() {
-        if (!mbar_wait(k_full + ks, kp, abort_flag)) return false;
-        tcgen05_fence_after();
+  // registers: 96 a thread at launch (5 x 96 = 480), dealt out anew: 2 x 128 + 2 x 80 + 64
+  if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    // ---------------- MMA issuers: the warp walks, an elected lane issues ----------------
+    const int i = warp - 16;
+    if (warp == 18) {
+      // ---------------- the share's items, in order (warp 19 makes the group whole) ----------------
+      PtWalk walk;
+      walk.b = s_b; walk.g = s_g; walk.j = s_j; walk.at = s_at; walk.begin = begin; walk.end = end;
+      walk.seq = pt_seq(p, walk.b);
+      PtItem x;
+      bool more = true;
+      for (int n = 0; more; ++n) {
+        more = walk.next(p, x);
+        if (!more) x.cols = 0;
+        const int at = n % kPtSlots;
+        ok = mbar_wait_relaxed(item_empty + at, ((n / kPtSlots) & 1) ^ 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) {
+          items[at] = x;
+          if (more && !x.whole && x.t_lo == 0) {
+            PagesRecord rec;
+            rec.pieces = (int)div_ll(walk.last_tile, (int)min(share, 0x7fffffffll)) - (int)blockIdx.x + 1;
+            rec.row0 = x.row0; rec.head0 = x.gh * p.hg; rec.col0 = x.col0;
+            rec.cols = x.cols;
+            p.records[blockIdx.x] = rec;
+          }
+          mbar_arrive(item_full + at);
+        }
+        __syncwarp();
+      }
+    }
+    int cols = 0, n = 0;
+    auto take = [&](const PtItem& x) { cols = x.cols; n = x.t_hi - x.t_lo; };
+    constexpr uint32_t idesc_s = pt_idesc(kPtKeys, false), idesc_o = pt_idesc(D, true);
+    const uint64_t q_desc = make_desc(smem_u32(smem + Cfg::kQ + i * Cfg::kTile), 16, 1024);
+    const uint64_t k_desc0 = make_desc(smem_u32(smem + Cfg::kK), 16, 1024);
+    const uint64_t v_desc0 = make_desc(smem_u32(smem + Cfg::kV), kPtSub, 1024);
+    const uint32_t s_col = tmem + Cfg::kColS + i * 128, o_col = tmem + Cfg::kColO + i * D;
+    int ks = 0, vs = 0, n_item = 0, t = 0;       // t: tiles of this half so far
+    uint32_t kp = 0, vp = 0;
+    auto next_k = [&]() { if (++ks == Cfg::kStages) { ks = 0; kp ^= 1; } };
+    auto next_v = [&]() { if (++vs == Cfg::kStages) { vs = 0; vp ^= 1; } };
+    auto issue_s = [&]() {
+      if (!mbar_wait(k_full + ks, kp, abort_flag)) return false;
+      __syncwarp();
+      tcgen05_fence_after();
+      if (elect_one()) {
         const uint64_t k_desc = k_desc0 + (uint64_t)((ks * Cfg::kTile) >> 4);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
@@ -302,130 +399,144 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
         }
         tcgen05_commit(k_empty + ks);
         tcgen05_commit(s_full + i);
-        next_k();
-        return true;
-      };
-      while (ok && walk.next(p, it)) {
-        const int n = it.t_hi - it.t_lo;
-        if (it.cols <= i * 128) {
-          // nothing for this half: the tiles are the other's alone
-          for (int u = 0; u < n && ok; ++u) {
-            ok = mbar_wait(k_full + ks, kp, abort_flag) && mbar_wait(v_full + vs, vp, abort_flag);
-            if (!ok) break;
+      }
+      __syncwarp();
+      next_k();
+      return true;
+    };
+    while (i < 2 && next_item(take)) {
+      if (cols <= i * 128) {
+        // nothing for this half: the tiles are the other's alone
+        for (int u = 0; u < n && ok; ++u) {
+          ok = mbar_wait(k_full + ks, kp, abort_flag) && mbar_wait(v_full + vs, vp, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (lane == 0) {
             mbar_arrive(k_empty + ks);
             mbar_arrive(v_empty + vs);
-            next_k(); next_v();
           }
-          continue;
+          next_k(); next_v();
         }
-        // the softmax's threads have written Q and read the last item's scores and outputs
-        ok = mbar_wait(q_full + i, n_item++ & 1, abort_flag) && issue_s();
-        for (int u = 0; u < n && ok; ++u, ++t) {
-          ok = mbar_wait(v_full + vs, vp, abort_flag) && mbar_wait(p_full + i, t & 1, abort_flag);
-          if (!ok) break;
-          tcgen05_fence_after();
+        continue;
+      }
+      // the softmax's threads have written Q; the last item's last product has read P
+      ok = mbar_wait(q_full + i, n_item & 1, abort_flag) && (t == 0 || mbar_wait(o_full + i, (t - 1) & 1, abort_flag)) &&
+           issue_s();
+      ok = __all_sync(0xffffffffu, ok);
+      // the last item's outputs have been read
+      if (ok && n_item > 0) ok = mbar_wait(o_free + i, (n_item - 1) & 1, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      ++n_item;
+      for (int u = 0; u < n && ok; ++u, ++t) {
+        ok = mbar_wait(v_full + vs, vp, abort_flag) && mbar_wait(p_full + i, t & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tcgen05_fence_after();
+        if (elect_one()) {
           const uint64_t v_desc = v_desc0 + (uint64_t)((vs * Cfg::kTile) >> 4);
 #pragma unroll
           for (int k = 0; k < kPtKeys / 16; ++k)
-            tcgen05_mma_ts(o_col, s_col + k * 8, v_desc + (uint64_t)((k * 16 * 128) >> 4), idesc_o, u > 0 || k != 0);
+            tcgen05_mma_ts(o_col, s_col + 64 + k * 8, v_desc + (uint64_t)((k * 16 * 128) >> 4), idesc_o, u > 0 || k != 0);
           tcgen05_commit(v_empty + vs);
           tcgen05_commit(o_full + i);
-          next_v();
-          if (u + 1 < n) {
-            // the next scores take P's place: the product that reads it must be done
-            ok = mbar_wait(o_full + i, t & 1, abort_flag) && issue_s();
-          }
+        }
+        __syncwarp();
+        next_v();
+        if (u + 1 < n) {
+          // the next scores take P's place: the product that reads it must be done
+          ok = mbar_wait(o_full + i, t & 1, abort_flag) && issue_s();
+          ok = __all_sync(0xffffffffu, ok);
         }
       }
     }
   } else if (warp >= 8) {
-    // ---------------- converters ----------------
-    // A thread has a 16-code piece of eight rows: rows 32 w + 4 r + lane / 8, so a load instruction
-    // takes whole 64- or 128-byte rows.  (With 64 codes a row, four pieces: rows 32 w + 8 r + lane / 4.)
+    // ---------------- converters: warps 8..11 the keys, 12..15 the values ----------------
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    // A thread has a 16-code piece of some rows.  A load instruction takes whole rows; eight
+    // lanes in a row, which store together, have four pieces of one sub-tile and two rows that
+    // differ in the swizzle's lowest bit, so their 16-byte stores meet on no bank.
     constexpr int kPieces = D / 16, kRowsAtOnce = 32 / kPieces, kReps = 32 / kRowsAtOnce;
-    const int w = warp - 8, piece = lane % kPieces, sub_row = lane / kPieces;
+    const bool values = warp >= 12;
+    const int w = warp & 3;
+    const int piece = (lane & 3) + (D == 128 ? (lane >> 3 & 1) * 4 : 0);
+    const int sub_row = (lane >> 2 & 1) + (D == 128 ? (lane >> 4) * 2 : (lane >> 3) * 2);
+    uint64_t* full = values ? v_full : k_full;
+    uint64_t* empty = values ? v_empty : k_empty;
+    uint8_t* tiles = smem + (values ? Cfg::kV : Cfg::kK);
     struct Tile { int key0, any_lo, any_hi, gh, entry; bool partial; };
-    Tile ahead;                    // the tile whose page ids are being looked up
+    PtItem it;
     int t_at = 0;
     bool have_item = false;
+    auto take = [&](const PtItem& x) { it = x; };
     auto advance = [&](Tile& x) {  // the next tile of the share; false at its end
       while (!have_item || t_at >= it.t_hi) {
-        if (!walk.next(p, it)) return false;
+        if (!next_item(take)) return false;
         have_item = true;
         t_at = it.t_lo;
       }
       x.key0 = (it.tile0 + t_at) * kPtKeys;
       x.any_lo = it.any_lo; x.any_hi = it.any_hi; x.gh = it.gh;
       x.partial = x.key0 < it.all_lo || x.key0 + kPtKeys > it.all_hi;
-      const int key = x.key0 + 32 * w + 16 * (lane & 1);      // even lanes: the warp's first page piece
-      int e = -1;
-      if (key < it.any_hi) e = p.tables[(long long)it.b * p.width + (key >> p.log_page)];
-      x.entry = e >= 0 && e < p.P ? e : -1;
+      const int key = x.key0 + 32 * w + 16 * (lane & 1);      // even lanes: the warp's first 16 keys
+      x.entry = -1;
+      if (key < it.any_hi) x.entry = p.tables[(long long)it.b * p.width + (key >> p.log_page)];
       ++t_at;
       return true;
     };
-    uint4 kr[kReps], vr[kReps];
-    const int page_mask = (1 << p.log_page) - 1;
-    auto base_of = [&](const Tile& x, int half, bool& there) {
-      const int e = __shfl_sync(0xffffffffu, x.entry, half);
-      there = e >= 0;
-      const int off = (x.key0 + 32 * w + 16 * half) & page_mask;
-      return p.pool + (((((long long)(there ? e : 0) * p.G + x.gh) * 2) << p.log_page) + off) * D;
-    };
-    auto load = [&](const Tile& x, bool values, uint4* r) {
+    uint4 codes[kReps];
+    // byte offsets of this thread's two 16-byte chunks: the swizzle's rows repeat every eight
+    const int at0 = (piece >> 2) * kPtSub + (32 * w + sub_row) * 128, chunk = 2 * (piece & 3);
+    const uint8_t* my_codes = p.pool + sub_row * D + piece * 16;
+    // A tile's page ids come as the index of a 16-token unit of one page, KV head and kind.
+    auto load = [&](const Tile& x) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        bool there;
-        const uint8_t* base = base_of(x, half, there) + (values ? ((long long)D << p.log_page) : 0);
+        const int unit = __shfl_sync(0xffffffffu, x.entry, half);
+        const uint8_t* base = my_codes + (long long)max(unit, 0) * (16 * D);
 #pragma unroll
         for (int k = 0; k < kReps / 2; ++k)
-          r[half * (kReps / 2) + k] = there ? ld_stream(base + (k * kRowsAtOnce + sub_row) * D + piece * 16) : make_uint4(0, 0, 0, 0);
+          codes[half * (kReps / 2) + k] = unit >= 0 ? ld_stream(base + k * kRowsAtOnce * D) : make_uint4(0, 0, 0, 0);
       }
     };
+    float2 scale = make_float2(1.f, 0.f);
+    auto unit_of = [&](Tile& x) {
+      const int off = (x.key0 + 32 * w + 16 * (lane & 1)) & ((1 << p.log_page) - 1);
+      const bool there = x.entry >= 0 && x.entry < p.P;
+      // an absent page: its scores are -inf through the logarithm, its share of the sum nothing
+      scale = make_float2(1.f, 0.f);
+      if (!values && there && lane < 2)
+        scale = *reinterpret_cast<const float2*>(p.scales + ((long long)x.entry * p.G + x.gh) * 2);
+      x.entry = there ? (((x.entry * p.G + x.gh) * 2 + (values ? 1 : 0)) << (p.log_page - 4)) + (off >> 4) : -1;
+    };
     auto store = [&](uint8_t* tile, int k, const uint4& c) {
-      const int row = 32 * w + k * kRowsAtOnce + sub_row, chunk = 2 * (piece & 3);
-      uint8_t* dst = tile + (piece >> 2) * kPtSub + row * 128;
+      const int row7 = (k * kRowsAtOnce + sub_row) & 7;
+      uint8_t* dst = tile + at0 + k * kRowsAtOnce * 128;
       uint4 lo, hi;
       halves16(c, lo, hi);
-      // the second sub-tile's lanes store their halves in the other order: no two lanes of a phase on one bank
-      const bool swap = D == 128 && (piece >> 2);
-      *reinterpret_cast<uint4*>(dst + (((chunk + (swap ? 1 : 0)) ^ (row & 7)) << 4)) = swap ? hi : lo;
-      *reinterpret_cast<uint4*>(dst + (((chunk + (swap ? 0 : 1)) ^ (row & 7)) << 4)) = swap ? lo : hi;
+      *reinterpret_cast<uint4*>(dst + ((chunk ^ row7) << 4)) = lo;
+      *reinterpret_cast<uint4*>(dst + (((chunk + 1) ^ row7) << 4)) = hi;
     };
     Tile now, nxt;
     bool have = advance(now), more = false;
     if (have) {
-      load(now, false, kr);
-      load(now, true, vr);
-      more = advance(nxt);
+      unit_of(now);
+      load(now);
+      more = advance(nxt);      // its page ids are there by the time its loads begin
     }
-    int s = 0;
+    int s = 0, n_tile = 0;
     uint32_t ph = 0;
-    while (have && ok) {
-      Tile after = nxt;
-      bool more_after = false;
-      ok = mbar_wait_relaxed(k_empty + s, ph ^ 1, abort_flag, 64);
+    while (have) {
+      ok = mbar_wait_relaxed(empty + s, ph ^ 1, abort_flag, 64);
+      ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      uint8_t* kt = smem + Cfg::kK + s * Cfg::kTile;
-#pragma unroll
-      for (int k = 0; k < kReps; ++k) store(kt, k, kr[k]);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(k_full + s);
-      if (more) {
-        load(nxt, false, kr);
-        more_after = advance(after);     // page ids of the tile after that
-      }
-      ok = mbar_wait_relaxed(v_empty + s, ph ^ 1, abort_flag, 64);
-      if (!ok) break;
-      uint8_t* vt = smem + Cfg::kV + s * Cfg::kTile;
-      if (now.partial) {
+      if (values && now.partial) {
         // values that no column sees count as zero; a NaN that some see is zero here and comes
         // back where it is seen when the outputs are written
 #pragma unroll
         for (int k = 0; k < kReps; ++k) {
           const int key = now.key0 + 32 * w + k * kRowsAtOnce + sub_row;
-          uint32_t* c = reinterpret_cast<uint32_t*>(&vr[k]);
-          if (key < now.any_lo || key >= now.any_hi) vr[k] = make_uint4(0, 0, 0, 0);
+          uint32_t* c = reinterpret_cast<uint32_t*>(&codes[k]);
+          if (key < now.any_lo || key >= now.any_hi) codes[k] = make_uint4(0, 0, 0, 0);
           if (nan_codes(c[0]) | nan_codes(c[1]) | nan_codes(c[2]) | nan_codes(c[3])) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) c[q] &= ~((nan_codes(c[q]) >> 7) * 0xffu);
@@ -433,116 +544,148 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
           }
         }
       }
+      if (!values) {
+        // the key scale, the logarithm of the value scale, its inverse: what the softmax asks for
+        const int at = n_tile++ % kPtScales;
+        if (lane < 2)
+          reinterpret_cast<float4*>(smem + Cfg::kScale)[at * 8 + 2 * w + lane] =
+              make_float4(scale.x, __log2f(scale.y), scale.y > 0.f ? __frcp_rn(scale.y) : 0.f, 0.f);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(scale_full + at);
+      }
+      uint8_t* tile = tiles + s * Cfg::kTile;
 #pragma unroll
-      for (int k = 0; k < kReps; ++k) store(vt, k, vr[k]);
+      for (int k = 0; k < kReps; ++k) store(tile, k, codes[k]);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(v_full + s);
-      if (more) load(nxt, true, vr);
+      mbar_arrive(full + s);
+      if (more) {
+        unit_of(nxt);
+        load(nxt);
+      }
       if (++s == Cfg::kStages) { s = 0; ph ^= 1; }
-      now = nxt; nxt = after;
-      have = more; more = more_after;
+      now = nxt;
+      have = more;
+      if (more) more = advance(nxt);
     }
   } else {
     // ---------------- softmax and output ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
     const int i = warp >> 2;                      // which 128 columns
     const int r = (warp & 3) * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t s_col = lanes + Cfg::kColS + i * 128, o_col = lanes + Cfg::kColO + i * D;
-    float4* scale_at = reinterpret_cast<float4*>(smem + Cfg::kScale) + warp * 16;
     uint8_t* q_row = smem + Cfg::kQ + i * Cfg::kTile + r * 128;
-    int t = 0;                                    // tiles of this half so far
-    while (ok && walk.next(p, it)) {
-      if (it.cols <= i * 128) continue;
-      const int c = it.col0 + i * 128 + r;        // column of the sequence and KV head
-      const bool live = i * 128 + r < it.cols;
-      const int row = c / p.hg, h = c - row * p.hg, pos = it.past + row;
-      const int hi_key = live ? (p.causal ? min(it.len, pos + 1) : it.len) : 0;
-      const int lo_key = p.window >= 0 ? pos - p.window : 0;
-      const long long out_at = ((long long)(it.row0 + row) * p.H + it.gh * p.hg + h) * D;
-      // ---- Q: halves under a power of two that puts the row's largest in [2^14, 2^15) ----
-      float factor;
-      {
-        const uint4* src = reinterpret_cast<const uint4*>(p.q + out_at);
-        uint4 raw[D / 8];
-#pragma unroll
-        for (int k = 0; k < D / 8; ++k) raw[k] = live ? ld_cached(src + k) : make_uint4(0, 0, 0, 0);
-        float mx = 0.f;
-#pragma unroll
-        for (int k = 0; k < D / 8; ++k) {
-          float f[8];
-          unpack8(raw[k], f);
-#pragma unroll
-          for (int q = 0; q < 8; ++q) mx = fmaxf(mx, fabsf(f[q]));
-        }
-        const int e = min(max((int)(__float_as_uint(mx) >> 23), 15), 254);
-        const float up = __uint_as_float((uint32_t)(268 - e) << 23);
-        factor = p.scale_log2 / up;
-#pragma unroll
-        for (int k = 0; k < D / 8; ++k) {
-          float f[8];
-          unpack8(raw[k], f);
-          *reinterpret_cast<uint4*>(q_row + (k >> 3) * kPtSub + (((k & 7) ^ (r & 7)) << 4)) =
-              make_uint4(pack_half2(f[0] * up, f[1] * up), pack_half2(f[2] * up, f[3] * up),
-                         pack_half2(f[4] * up, f[5] * up), pack_half2(f[6] * up, f[7] * up));
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        tcgen05_fence_before();      // the last item's scores and outputs have been read
-        mbar_arrive(q_full + i);
+    int t = 0, n_tile = 0;                        // tiles of this half, and of the share, so far
+    PtItem it;
+    // what a thread keeps of its column
+    struct Row { long long out_at; float factor; int hi_key, lo_key; bool live; } me;
+    auto take = [&](const PtItem& x) { it = x; };
+    // The next item with columns for this half, and its queries: halves under a power of two that
+    // puts the row's largest in [2^14, 2^15).  The last item's scores have been computed, so Q's
+    // place is free; its outputs may still be to come.
+    auto open_item = [&]() {
+      for (;;) {
+        if (!next_item(take)) return false;
+        if (it.cols > i * 128) break;
+        n_tile += it.t_hi - it.t_lo;
       }
-      // ---- scales: lanes 0 .. 7 have a 16-key unit each, ids two tiles ahead, scales one ----
-      const int* table = p.tables + (long long)it.b * p.width;
-      auto entry_of = [&](int tile) {
-        const int key = (it.tile0 + tile) * kPtKeys + 16 * (lane & 7);
-        int e = -1;
-        if (tile < it.t_hi && key < it.any_hi) e = table[key >> p.log_page];
-        return e >= 0 && e < p.P ? e : -1;
-      };
-      auto scale_of = [&](int e) {
-        return e >= 0 ? *reinterpret_cast<const float2*>(p.scales + ((long long)e * p.G + it.gh) * 2) : make_float2(1.f, 0.f);
-      };
-      int e1 = entry_of(it.t_lo);
-      float2 sc = scale_of(e1);
-      e1 = entry_of(it.t_lo + 1);
+      const int c = it.col0 + i * 128 + r;        // column of the sequence and KV head
+      const int row = c / p.hg, h = c - row * p.hg, pos = it.past + row;
+      me.live = i * 128 + r < it.cols;
+      me.hi_key = me.live ? (p.causal ? min(it.len, pos + 1) : it.len) : 0;
+      me.lo_key = p.window >= 0 ? pos - p.window : 0;
+      me.out_at = ((long long)(it.row0 + row) * p.H + it.gh * p.hg + h) * D;
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + me.out_at);
+      uint4 raw[D / 8];
+#pragma unroll
+      for (int k = 0; k < D / 8; ++k) raw[k] = me.live ? ld_cached(src + k) : make_uint4(0, 0, 0, 0);
+      // the largest magnitude, two elements at a time: bf16 magnitudes order as their bits do
+      uint32_t top = 0;
+#pragma unroll
+      for (int k = 0; k < D / 8; ++k) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[k]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) top = __vmaxu2(top, w[q] & 0x7fff7fffu);
+      }
+      const float mx = __uint_as_float(max(top & 0xffffu, top >> 16) << 16);
+      const int e = min(max((int)(__float_as_uint(mx) >> 23), 15), 254);
+      const float up = __uint_as_float((uint32_t)(268 - e) << 23);
+      me.factor = p.scale_log2 / up;
+#pragma unroll
+      for (int k = 0; k < D / 8; ++k) {
+        float f[8];
+        unpack8(raw[k], f);
+        *reinterpret_cast<uint4*>(q_row + (k >> 3) * kPtSub + (((k & 7) ^ (r & 7)) << 4)) =
+            make_uint4(pack_half2(f[0] * up, f[1] * up), pack_half2(f[2] * up, f[3] * up),
+                       pack_half2(f[4] * up, f[5] * up), pack_half2(f[6] * up, f[7] * up));
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(q_full + i);
+      return true;
+    };
+    // 64 bytes of each lane's row in: 16 bytes of rows 8 k + lane / 4 out, k = 0 .. 3.
+    auto turn_rows = [&](uint32_t* o) {
+      uint8_t* mine = smem + Cfg::kOut + warp * 32 * kPtPitch;
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        *reinterpret_cast<uint4*>(mine + lane * kPtPitch + k * 16) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint4 x = *reinterpret_cast<const uint4*>(mine + (8 * k + (lane >> 2)) * kPtPitch + (lane & 3) * 16);
+        o[4 * k] = x.x; o[4 * k + 1] = x.y; o[4 * k + 2] = x.z; o[4 * k + 3] = x.w;
+      }
+    };
+    bool have = open_item();
+    while (have) {
+      const float factor = me.factor;
+      const int hi_key = me.hi_key, lo_key = me.lo_key;
       float m_used = -INFINITY, l = 0.f;
 
-      for (int u = it.t_lo; u < it.t_hi && ok; ++u, ++t) {
-        if (lane < 8) {
-          // an absent page: its scores are -inf through the logarithm, its share of the sum nothing
-          scale_at[(u & 1) * 8 + lane] = make_float4(sc.x, __log2f(sc.y), sc.y > 0.f ? 1.f / sc.y : 0.f, 0.f);
-        }
-        __syncwarp();
-        sc = scale_of(e1);
-        e1 = entry_of(u + 2);
-        const uint32_t sc_at = smem_u32(scale_at + (u & 1) * 8);
+      for (int u = it.t_lo; u < it.t_hi && ok; ++u, ++t, ++n_tile) {
+        const uint32_t sc_at = smem_u32(smem + Cfg::kScale) + (n_tile % kPtScales) * 128;
         const int key0 = (it.tile0 + u) * kPtKeys;
         const bool partial = key0 < it.all_lo || key0 + kPtKeys > it.all_hi;
-        ok = mbar_wait(s_full + i, t & 1, abort_flag);
+        ok = mbar_wait(scale_full + n_tile % kPtScales, (n_tile / kPtScales) & 1, abort_flag) &&
+             mbar_wait(s_full + i, t & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tcgen05_fence_after();
-        auto mask = [&](uint32_t* v, int first) {     // scores of keys first .. first + 31 this column does not see
-#pragma unroll
-          for (int k = 0; k < 32; ++k)
-            if (first + k >= hi_key || first + k < lo_key) v[k] = 0xff800000u;
-        };
-        // ---- the maximum ----
-        float mx = -INFINITY;
         uint32_t v[2][32];
+        if (partial) {
+          // scores of keys this column does not see become -inf where they lie
+#pragma unroll 1
+          for (int q = 0; q < 4; ++q) {
+            tmem_ld32(s_col + q * 32, v[0]);
+            tmem_ld_wait32(v[0]);
+            const int first = key0 + q * 32;
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (first + k >= hi_key || first + k < lo_key) v[0][k] = 0xff800000u;
+            tmem_st16(s_col + q * 32, v[0]);
+            tmem_st16(s_col + q * 32 + 16, v[0] + 16);
+          }
+          tmem_st_wait();
+        }
+        // ---- the maximum: the next 32 scores come while these are looked at ----
+        float mx = -INFINITY;
         tmem_ld32(s_col, v[0]);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          tmem_ld_wait();
+          const uint4 f0 = pt_lds128(sc_at + q * 32), f1 = pt_lds128(sc_at + q * 32 + 16);
+          tmem_ld_wait32(v[q & 1]);
           if (q < 3) tmem_ld32(s_col + (q + 1) * 32, v[(q + 1) & 1]);
-          uint32_t* x = v[q & 1];
-          if (partial) mask(x, key0 + q * 32);
+          const uint32_t* x = v[q & 1];
+          float top0 = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+          float top1 = fmaxf(__uint_as_float(x[16]), __uint_as_float(x[17]));
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            float top = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < 16; ++k) top = fmaxf(top, __uint_as_float(x[half * 16 + k]));
-            const uint4 f = pt_lds128(sc_at + (q * 2 + half) * 16);
-            mx = fmaxf(mx, fmaf(top, score_factor(factor, f.x), __uint_as_float(f.y)));
+          for (int k = 2; k < 16; k += 2) {
+            top0 = max3(top0, __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+            top1 = max3(top1, __uint_as_float(x[16 + k]), __uint_as_float(x[17 + k]));
           }
+          mx = max3(mx, fmaf(top0, score_factor(factor, f0.x), __uint_as_float(f0.y)),
+                    fmaf(top1, score_factor(factor, f1.x), __uint_as_float(f1.y)));
         }
         if (__any_sync(0xffffffffu, mx > m_used + kPtSlack)) {
           const float m_new = fmaxf(m_used, mx);
@@ -551,10 +694,10 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
           l *= corr;
           if (u > it.t_lo) {
             // the scores of this tile came after the last tile's product: the outputs lie still
-#pragma unroll
+#pragma unroll 1
             for (int q = 0; q < D / 32; ++q) {
               tmem_ld32(o_col + q * 32, v[0]);
-              tmem_ld_wait();
+              tmem_ld_wait32(v[0]);
 #pragma unroll
               for (int k = 0; k < 32; ++k) v[0][k] = __float_as_uint(__uint_as_float(v[0][k]) * corr);
               tmem_st16(o_col + q * 32, v[0]);
@@ -564,43 +707,48 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
         }
         // ---- weights: P over the scores' place, and their sum ----
         const float base = (m_used == -INFINITY ? 0.f : m_used) - kPtLift;
-        tmem_ld32(s_col, v[0]);
+        // From the last scores, which are here, to the first: columns 64 + 16 q .. of P lie on scores
+        // that have been read.
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          tmem_ld_wait();
-          if (q < 3) tmem_ld32(s_col + (q + 1) * 32, v[(q + 1) & 1]);
-          uint32_t* x = v[q & 1];
-          if (partial) mask(x, key0 + q * 32);
+        for (int q = 3; q >= 0; --q) {
+          const uint4 f0 = pt_lds128(sc_at + q * 32), f1 = pt_lds128(sc_at + q * 32 + 16);
+          if (q < 3) tmem_ld_wait32(v[q & 1]);
+          if (q > 0) tmem_ld32(s_col + (q - 1) * 32, v[(q - 1) & 1]);
+          const uint32_t* x = v[q & 1];
           uint32_t out[16];
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const uint4 f = pt_lds128(sc_at + (q * 2 + half) * 16);
+            const uint4& f = half ? f1 : f0;
             const float a = score_factor(factor, f.x), b = __uint_as_float(f.y) - base;
-            float sum0 = 0.f, sum1 = 0.f;
+            const uint64_t a2 = pair(a, a), b2 = pair(b, b);
+            uint64_t sum[2] = {0, 0};
 #pragma unroll
             for (int k = 0; k < 16; k += 2) {
-              const float p0 = ex2(fmaf(__uint_as_float(x[half * 16 + k]), a, b));
-              const float p1 = ex2(fmaf(__uint_as_float(x[half * 16 + k + 1]), a, b));
-              sum0 += p0; sum1 += p1;
+              const float2 y = unpair(fma2(pair(__uint_as_float(x[half * 16 + k]), __uint_as_float(x[half * 16 + k + 1])), a2, b2));
+              const float p0 = ex2(y.x), p1 = ex2(y.y);
+              sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], pair(p0, p1));
               out[half * 8 + k / 2] = pack_half2(p0, p1);
             }
-            l = fmaf(sum0 + sum1, __uint_as_float(f.z), l);
+            const float2 total = unpair(add2(sum[0], sum[1]));
+            l = fmaf(total.x + total.y, __uint_as_float(f.z), l);
           }
-          // columns 16 q .. of P lie on scores that have been read: 16 q + 16 <= 32 (q + 1)
-          if (q < 3) tmem_ld_wait();
-          tmem_st16(s_col + q * 16, out);
+          tmem_st16(s_col + 64 + q * 16, out);
         }
         tmem_st_wait();
         tcgen05_fence_before();
         mbar_arrive(p_full + i);
       }
-      // ---- the item's results ----
-      if (ok) ok = mbar_wait(o_full + i, (t - 1) & 1, abort_flag);
+      if (!ok) break;
+      // ---- the next item's queries go first, then this one's results ----
+      const PtItem done = it;
+      const Row was = me;
+      const int last = t - 1;
+      have = open_item();
+      ok = ok && mbar_wait(o_full + i, last & 1, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tcgen05_fence_after();
-      const bool direct = it.t_lo == 0 && it.t_hi == it.tiles;
-      float* part = p.partial + ((long long)blockIdx.x * 2 + (it.t_lo == 0 ? 1 : 0)) * Cfg::kPartial;
+      float* part = p.partial + ((long long)blockIdx.x * 2 + (done.t_lo == 0 ? 1 : 0)) * Cfg::kPartial;
       const bool nans = *reinterpret_cast<volatile int*>(&s_nan) != 0;
       const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
@@ -608,17 +756,21 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
         uint32_t v[32];
         __syncwarp();
         tmem_ld32(o_col + q * 32, v);
-        tmem_ld_wait();
-        if (nans && live) {
+        tmem_ld_wait32(v);
+        if (q == D / 32 - 1) {
+          tcgen05_fence_before();
+          mbar_arrive(o_free + i);     // the outputs are read: the next item's may come
+        }
+        if (nans && was.live) {
           // NaN codes of partial tiles were taken as zero: they are NaN to the rows that see them
           uint32_t hit = 0;
-          const int from = max(lo_key, (it.tile0 + it.t_lo) * kPtKeys), to = min(hi_key, (it.tile0 + it.t_hi) * kPtKeys);
+          const int from = max(was.lo_key, (done.tile0 + done.t_lo) * kPtKeys), to = min(was.hi_key, (done.tile0 + done.t_hi) * kPtKeys);
           for (int key = max(from, 0); key < to; ++key) {
             const int k0 = key / kPtKeys * kPtKeys;
-            if (k0 >= it.all_lo && k0 + kPtKeys <= it.all_hi) { key = k0 + kPtKeys - 1; continue; }
-            const int e = table[key >> p.log_page];
+            if (k0 >= done.all_lo && k0 + kPtKeys <= done.all_hi) { key = k0 + kPtKeys - 1; continue; }
+            const int e = p.tables[(long long)done.b * p.width + (key >> p.log_page)];
             if (e < 0 || e >= p.P) continue;
-            const long long block = ((long long)e * p.G + it.gh) * 2 + 1;
+            const long long block = ((long long)e * p.G + done.gh) * 2 + 1;
             const uint32_t* code = reinterpret_cast<const uint32_t*>(
                 p.pool + ((block << p.log_page) + (key & ((1 << p.log_page) - 1))) * D + q * 32);
             for (int k = 0; k < 8; ++k) {
@@ -630,38 +782,43 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
           for (int k = 0; k < 32; ++k)
             if (hit >> k & 1) v[k] = 0x7fc00000u;
         }
-        if (live && direct) {
+        // A lane has 32 columns of its row; through shared memory four lanes have 64 bytes of one, so
+        // that a store instruction writes eight rows' pieces instead of 32 rows'.
+        if (done.whole) {
           uint32_t o[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k)
             o[k] = l == 0.f ? 0u : pack_bf16x2(__uint_as_float(v[2 * k]) * inv, __uint_as_float(v[2 * k + 1]) * inv);
+          turn_rows(o);
 #pragma unroll
-          for (int k = 0; k < 16; k += 4)
-            *reinterpret_cast<uint4*>(p.out + out_at + q * 32 + 2 * k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-        } else if (live) {
+          for (int k = 0; k < 4; ++k) {
+            const long long at = __shfl_sync(0xffffffffu, was.out_at, 8 * k + (lane >> 2));
+            if (__shfl_sync(0xffffffffu, was.live ? 1 : 0, 8 * k + (lane >> 2)))
+              *reinterpret_cast<uint4*>(p.out + at + q * 32 + (lane & 3) * 8) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          }
+        } else {
 #pragma unroll
-          for (int k = 0; k < 32; k += 4)
-            *reinterpret_cast<uint4*>(part + (i * 128 + r) * D + q * 32 + k) = make_uint4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+          for (int half = 0; half < 2; ++half) {
+            uint32_t* o = v + half * 16;
+            turn_rows(o);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int row = (warp & 3) * 32 + 8 * k + (lane >> 2);
+              if (i * 128 + row < done.cols)
+                *reinterpret_cast<uint4*>(part + (i * 128 + row) * D + q * 32 + half * 16 + (lane & 3) * 4) =
+                    make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+            }
+          }
         }
       }
-      if (!direct) {
-        if (live) {
-          part[kPtRows * D + i * 128 + r] = m_used;
-          part[kPtRows * D + kPtRows + i * 128 + r] = l;
-        }
-        if (tid == 0 && it.t_lo == 0) {
-          const int w = it.cols > 128 ? 2 : 1;
-          PagesRecord rec;
-          rec.pieces = (int)((it.at + kPtItemCost + (long long)(it.tiles - 1) * w) / share) - (int)blockIdx.x + 1;
-          rec.row0 = it.row0; rec.head0 = it.gh * p.hg; rec.col0 = it.col0;
-          rec.cols = it.cols;
-          p.records[blockIdx.x] = rec;
-        }
+      if (was.live && !done.whole) {
+        part[kPtRows * D + i * 128 + r] = m_used;
+        part[kPtRows * D + kPtRows + i * 128 + r] = l;
       }
     }
   }
 
-  if (!ok) {
+  if (*abort_flag) {
     // a wait gave up: give what is in flight a millisecond, many times what it takes
     const unsigned long long t0 = global_ns();
     while (global_ns() - t0 < 1000000ull) {}
@@ -669,7 +826,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
   tcgen05_fence_before();
   __syncthreads();
   if (tid == 0 && *abort_flag && p.status) *p.status = IRON_ERR_TIMEOUT;
-  if (warp == 12) {
+  if (warp == 16) {
     tcgen05_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
