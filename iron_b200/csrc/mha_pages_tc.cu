@@ -63,7 +63,7 @@ struct PtCfg {
   static constexpr int kOut = kItems + kPtSlots * 64;      // [8 warps] 32 rows x 64 bytes, kPtPitch apart
   static constexpr int kBars = kOut + 8 * 32 * kPtPitch;
   static constexpr int kSmem = kBars + 512 + 1024;
-  static constexpr int kColS = 0;                          // 2 x 128 columns (P: the last 64 of each)
+  static constexpr int kColS = 0;                          // 2 halves x 2 buffers x 64 columns (P: the last 32 of each)
   static constexpr int kColO = 256;                        // 2 x D columns
   static constexpr int kPartial = kPtRows * (D + 2);       // floats: outputs, maxima, sums
 };
@@ -154,6 +154,17 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
         "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+// Sixteen columns, waited for.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // The second product: A in tensor memory (row = lane, two halves of K per 32-bit column).
 __device__ __forceinline__ void tcgen05_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
@@ -228,10 +239,10 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
   uint64_t* v_full = k_empty + Cfg::kStages;
   uint64_t* v_empty = v_full + Cfg::kStages;
   uint64_t* q_full = v_empty + Cfg::kStages;        // [2] each: one a half of the columns
-  uint64_t* s_full = q_full + 2;
-  uint64_t* p_full = s_full + 2;
-  uint64_t* o_full = p_full + 2;
-  uint64_t* o_free = o_full + 2;
+  uint64_t* s_full = q_full + 2;                    // [2][2]: of a half's two buffers
+  uint64_t* p_full = s_full + 4;                    // [2][2]
+  uint64_t* o_full = p_full + 4;                    // [2][2]: a step's product is done, by the buffer its P lay in
+  uint64_t* o_free = o_full + 4;                    // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_free + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint64_t* item_full = o_free + 3;                 // [kPtSlots] each (behind the two words above)
@@ -306,7 +317,10 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
       mbar_init(k_full + s, 128); mbar_init(k_empty + s, 2); mbar_init(v_full + s, 128); mbar_init(v_empty + s, 2);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(q_full + i, 128); mbar_init(s_full + i, 1); mbar_init(p_full + i, 128); mbar_init(o_full + i, 1);
+      mbar_init(q_full + i, 128);
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(s_full + 2 * i + k, 1); mbar_init(p_full + 2 * i + k, 128); mbar_init(o_full + 2 * i + k, 1);
+      }
       mbar_init(o_free + i, 128);
     }
     for (int s = 0; s < kPtSlots; ++s) { mbar_init(item_full + s, 1); mbar_init(item_empty + s, kPtRoles); }
@@ -377,33 +391,38 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
     }
     int cols = 0, n = 0;
     auto take = [&](const PtItem& x) { cols = x.cols; n = x.t_hi - x.t_lo; };
-    constexpr uint32_t idesc_s = pt_idesc(kPtKeys, false), idesc_o = pt_idesc(D, true);
+    constexpr uint32_t idesc_s = pt_idesc(64, false), idesc_o = pt_idesc(D, true);
     const uint64_t q_desc = make_desc(smem_u32(smem + Cfg::kQ + i * Cfg::kTile), 16, 1024);
     const uint64_t k_desc0 = make_desc(smem_u32(smem + Cfg::kK), 16, 1024);
     const uint64_t v_desc0 = make_desc(smem_u32(smem + Cfg::kV), kPtSub, 1024);
     const uint32_t s_col = tmem + Cfg::kColS + i * 128, o_col = tmem + Cfg::kColO + i * D;
-    int ks = 0, vs = 0, n_item = 0, t = 0;       // t: tiles of this half so far
+    // A tile goes in two steps of 64 keys: while a step's exponentials are taken, the next one's
+    // scores are computed into the other buffer.  t, t_s: steps of this half so far, and scores issued.
+    int ks = 0, vs = 0, n_item = 0, t = 0, t_s = 0;
     uint32_t kp = 0, vp = 0;
     auto next_k = [&]() { if (++ks == Cfg::kStages) { ks = 0; kp ^= 1; } };
     auto next_v = [&]() { if (++vs == Cfg::kStages) { vs = 0; vp ^= 1; } };
     auto issue_s = [&]() {
-      if (!mbar_wait(k_full + ks, kp, abort_flag)) return false;
+      const int sub = t_s & 1;
+      if (sub == 0 && !mbar_wait(k_full + ks, kp, abort_flag)) return false;
       __syncwarp();
       tcgen05_fence_after();
       if (elect_one()) {
-        const uint64_t k_desc = k_desc0 + (uint64_t)((ks * Cfg::kTile) >> 4);
+        const uint64_t k_desc = k_desc0 + (uint64_t)((ks * Cfg::kTile + sub * 64 * 128) >> 4);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint64_t off = (uint64_t)((k >> 2) * (kPtSub >> 4) + (k & 3) * 2);
-          tcgen05_mma_bf16(s_col, q_desc + off, k_desc + off, idesc_s, k != 0);
+          tcgen05_mma_bf16(s_col + sub * 64, q_desc + off, k_desc + off, idesc_s, k != 0);
         }
-        tcgen05_commit(k_empty + ks);
-        tcgen05_commit(s_full + i);
+        if (sub) tcgen05_commit(k_empty + ks);
+        tcgen05_commit(s_full + 2 * i + sub);
       }
       __syncwarp();
-      next_k();
+      if (sub) next_k();
+      ++t_s;
       return true;
     };
+    auto o_done = [&](int step) { return mbar_wait(o_full + 2 * i + (step & 1), (step >> 1) & 1, abort_flag); };
     while (i < 2 && next_item(take)) {
       if (cols <= i * 128) {
         // nothing for this half: the tiles are the other's alone
@@ -420,31 +439,32 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
         continue;
       }
       // the softmax's threads have written Q; the last item's last product has read P
-      ok = mbar_wait(q_full + i, n_item & 1, abort_flag) && (t == 0 || mbar_wait(o_full + i, (t - 1) & 1, abort_flag)) &&
-           issue_s();
+      ok = mbar_wait(q_full + i, n_item & 1, abort_flag) && (t == 0 || o_done(t - 1)) && issue_s() && issue_s();
       ok = __all_sync(0xffffffffu, ok);
       // the last item's outputs have been read
       if (ok && n_item > 0) ok = mbar_wait(o_free + i, (n_item - 1) & 1, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       ++n_item;
-      for (int u = 0; u < n && ok; ++u, ++t) {
-        ok = mbar_wait(v_full + vs, vp, abort_flag) && mbar_wait(p_full + i, t & 1, abort_flag);
+      for (int u = 0; u < 2 * n && ok; ++u, ++t) {
+        const int sub = u & 1;
+        ok = (sub || mbar_wait(v_full + vs, vp, abort_flag)) && mbar_wait(p_full + 2 * i + sub, (t >> 1) & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tcgen05_fence_after();
         if (elect_one()) {
-          const uint64_t v_desc = v_desc0 + (uint64_t)((vs * Cfg::kTile) >> 4);
+          const uint64_t v_desc = v_desc0 + (uint64_t)((vs * Cfg::kTile + sub * 64 * 128) >> 4);
 #pragma unroll
-          for (int k = 0; k < kPtKeys / 16; ++k)
-            tcgen05_mma_ts(o_col, s_col + 64 + k * 8, v_desc + (uint64_t)((k * 16 * 128) >> 4), idesc_o, u > 0 || k != 0);
-          tcgen05_commit(v_empty + vs);
-          tcgen05_commit(o_full + i);
+          for (int k = 0; k < 4; ++k)
+            tcgen05_mma_ts(o_col, s_col + sub * 64 + 32 + k * 8, v_desc + (uint64_t)((k * 16 * 128) >> 4), idesc_o,
+                           u > 0 || k != 0);
+          if (sub) tcgen05_commit(v_empty + vs);
+          tcgen05_commit(o_full + 2 * i + sub);
         }
         __syncwarp();
-        next_v();
-        if (u + 1 < n) {
-          // the next scores take P's place: the product that reads it must be done
-          ok = mbar_wait(o_full + i, t & 1, abort_flag) && issue_s();
+        if (sub) next_v();
+        if (u + 2 < 2 * n) {
+          // the scores after the next take this step's place: the product that reads its P must be done
+          ok = o_done(t) && issue_s();
           ok = __all_sync(0xffffffffu, ok);
         }
       }
@@ -575,7 +595,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t s_col = lanes + Cfg::kColS + i * 128, o_col = lanes + Cfg::kColO + i * D;
     uint8_t* q_row = smem + Cfg::kQ + i * Cfg::kTile + r * 128;
-    int t = 0, n_tile = 0;                        // tiles of this half, and of the share, so far
+    int t = 0, n_tile = 0;                        // steps of this half, and tiles of the share, so far
     PtItem it;
     // what a thread keeps of its column
     struct Row { long long out_at; float factor; int hi_key, lo_key; bool live; } me;
@@ -643,100 +663,86 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
       const int hi_key = me.hi_key, lo_key = me.lo_key;
       float m_used = -INFINITY, l = 0.f;
 
-      for (int u = it.t_lo; u < it.t_hi && ok; ++u, ++t, ++n_tile) {
-        const uint32_t sc_at = smem_u32(smem + Cfg::kScale) + (n_tile % kPtScales) * 128;
-        const int key0 = (it.tile0 + u) * kPtKeys;
-        const bool partial = key0 < it.all_lo || key0 + kPtKeys > it.all_hi;
-        ok = mbar_wait(scale_full + n_tile % kPtScales, (n_tile / kPtScales) & 1, abort_flag) &&
-             mbar_wait(s_full + i, t & 1, abort_flag);
+      for (int u = 2 * it.t_lo; u < 2 * it.t_hi && ok; ++u, ++t) {
+        const int sub = u & 1, buf = 2 * i + sub;
+        const uint32_t col = s_col + sub * 64;
+        const uint32_t sc_at = smem_u32(smem + Cfg::kScale) + (n_tile % kPtScales) * 128 + sub * 64;
+        const int key0 = it.tile0 * kPtKeys + u * 64;
+        ok = (sub || mbar_wait(scale_full + n_tile % kPtScales, (n_tile / kPtScales) & 1, abort_flag)) &&
+             mbar_wait(s_full + buf, (t >> 1) & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
+        if (sub) ++n_tile;
         tcgen05_fence_after();
-        uint32_t v[2][32];
-        if (partial) {
-          // scores of keys this column does not see become -inf where they lie
-#pragma unroll 1
-          for (int q = 0; q < 4; ++q) {
-            tmem_ld32(s_col + q * 32, v[0]);
-            tmem_ld_wait32(v[0]);
-            const int first = key0 + q * 32;
+        uint32_t v[64];
+        tmem_ld32(col, v);
+        tmem_ld32(col + 32, v + 32);
+        // (key scale, log2 of the value scale, its inverse) of each 16 keys
+        const uint4 f[4] = {pt_lds128(sc_at), pt_lds128(sc_at + 16), pt_lds128(sc_at + 32), pt_lds128(sc_at + 48)};
+        tmem_ld_wait32(v);
+        tmem_ld_wait32(v + 32);
+        if (key0 < it.all_lo || key0 + 64 > it.all_hi) {
 #pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (first + k >= hi_key || first + k < lo_key) v[0][k] = 0xff800000u;
-            tmem_st16(s_col + q * 32, v[0]);
-            tmem_st16(s_col + q * 32 + 16, v[0] + 16);
-          }
-          tmem_st_wait();
+          for (int k = 0; k < 64; ++k)
+            if (key0 + k >= hi_key || key0 + k < lo_key) v[k] = 0xff800000u;   // this column does not see the key
         }
-        // ---- the maximum: the next 32 scores come while these are looked at ----
+        // ---- the maximum ----
         float mx = -INFINITY;
-        tmem_ld32(s_col, v[0]);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const uint4 f0 = pt_lds128(sc_at + q * 32), f1 = pt_lds128(sc_at + q * 32 + 16);
-          tmem_ld_wait32(v[q & 1]);
-          if (q < 3) tmem_ld32(s_col + (q + 1) * 32, v[(q + 1) & 1]);
-          const uint32_t* x = v[q & 1];
-          float top0 = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-          float top1 = fmaxf(__uint_as_float(x[16]), __uint_as_float(x[17]));
+          float top = fmaxf(__uint_as_float(v[16 * q]), __uint_as_float(v[16 * q + 1]));
 #pragma unroll
-          for (int k = 2; k < 16; k += 2) {
-            top0 = max3(top0, __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
-            top1 = max3(top1, __uint_as_float(x[16 + k]), __uint_as_float(x[17 + k]));
-          }
-          mx = max3(mx, fmaf(top0, score_factor(factor, f0.x), __uint_as_float(f0.y)),
-                    fmaf(top1, score_factor(factor, f1.x), __uint_as_float(f1.y)));
+          for (int k = 2; k < 16; k += 2) top = max3(top, __uint_as_float(v[16 * q + k]), __uint_as_float(v[16 * q + k + 1]));
+          mx = fmaxf(mx, fmaf(top, score_factor(factor, f[q].x), __uint_as_float(f[q].y)));
         }
         if (__any_sync(0xffffffffu, mx > m_used + kPtSlack)) {
           const float m_new = fmaxf(m_used, mx);
           const float corr = m_new == -INFINITY ? 1.f : ex2(m_used - m_new);
           m_used = m_new;
           l *= corr;
-          if (u > it.t_lo) {
-            // the scores of this tile came after the last tile's product: the outputs lie still
+          if (u > 2 * it.t_lo) {
+            // once the last step's product is done the outputs lie still: this step's waits for P.
+            // (These scores took the place of the step before's P: its product is done.)
+            ok = mbar_wait(o_full + 2 * i + ((t - 1) & 1), ((t - 1) >> 1) & 1, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tcgen05_fence_after();
 #pragma unroll 1
-            for (int q = 0; q < D / 32; ++q) {
-              tmem_ld32(o_col + q * 32, v[0]);
-              tmem_ld_wait32(v[0]);
+            for (int q = 0; q < D / 16; ++q) {
+              uint32_t o[16];
+              tmem_ld16(o_col + q * 16, o);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) v[0][k] = __float_as_uint(__uint_as_float(v[0][k]) * corr);
-              tmem_st16(o_col + q * 32, v[0]);
-              tmem_st16(o_col + q * 32 + 16, v[0] + 16);
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * corr);
+              tmem_st16(o_col + q * 16, o);
             }
           }
         }
-        // ---- weights: P over the scores' place, and their sum ----
+        // ---- weights and their sum: P over the scores' place ----
         const float base = (m_used == -INFINITY ? 0.f : m_used) - kPtLift;
-        // From the last scores, which are here, to the first: columns 64 + 16 q .. of P lie on scores
-        // that have been read.
 #pragma unroll
-        for (int q = 3; q >= 0; --q) {
-          const uint4 f0 = pt_lds128(sc_at + q * 32), f1 = pt_lds128(sc_at + q * 32 + 16);
-          if (q < 3) tmem_ld_wait32(v[q & 1]);
-          if (q > 0) tmem_ld32(s_col + (q - 1) * 32, v[(q - 1) & 1]);
-          const uint32_t* x = v[q & 1];
+        for (int half = 0; half < 2; ++half) {
           uint32_t out[16];
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint4& f = half ? f1 : f0;
-            const float a = score_factor(factor, f.x), b = __uint_as_float(f.y) - base;
+          for (int qq = 0; qq < 2; ++qq) {
+            const int q = 2 * half + qq;
+            const float a = score_factor(factor, f[q].x), b = __uint_as_float(f[q].y) - base;
             const uint64_t a2 = pair(a, a), b2 = pair(b, b);
             uint64_t sum[2] = {0, 0};
 #pragma unroll
             for (int k = 0; k < 16; k += 2) {
-              const float2 y = unpair(fma2(pair(__uint_as_float(x[half * 16 + k]), __uint_as_float(x[half * 16 + k + 1])), a2, b2));
+              const float2 y = unpair(fma2(pair(__uint_as_float(v[16 * q + k]), __uint_as_float(v[16 * q + k + 1])), a2, b2));
               const float p0 = ex2(y.x), p1 = ex2(y.y);
               sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], pair(p0, p1));
-              out[half * 8 + k / 2] = pack_half2(p0, p1);
+              out[qq * 8 + k / 2] = pack_half2(p0, p1);
             }
             const float2 total = unpair(add2(sum[0], sum[1]));
-            l = fmaf(total.x + total.y, __uint_as_float(f.z), l);
+            l = fmaf(total.x + total.y, __uint_as_float(f[q].z), l);
           }
-          tmem_st16(s_col + 64 + q * 16, out);
+          tmem_st16(col + 32 + half * 16, out);
         }
         tmem_st_wait();
         tcgen05_fence_before();
-        mbar_arrive(p_full + i);
+        mbar_arrive(p_full + buf);
       }
       if (!ok) break;
       // ---- the next item's queries go first, then this one's results ----
@@ -744,7 +750,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
       const Row was = me;
       const int last = t - 1;
       have = open_item();
-      ok = ok && mbar_wait(o_full + i, last & 1, abort_flag);
+      ok = ok && mbar_wait(o_full + 2 * i + (last & 1), (last >> 1) & 1, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tcgen05_fence_after();
