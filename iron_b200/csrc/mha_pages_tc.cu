@@ -40,7 +40,7 @@ constexpr int kPtKeys = 128;          // keys of a tile
 constexpr int kPtSub = 16384;         // a 128-row x 128-byte swizzled sub-tile
 // What the tiles of one and of two 128-column halves cost, and an item beside its tiles, as measured:
 // one half alone waits for its own chain of products and exponentials.
-constexpr int kPtCostOne = 4, kPtCostTwo = 6, kPtItemCost = 12;
+constexpr int kPtCostOne = 3, kPtCostTwo = 4, kPtItemCost = 12;
 constexpr int kPtMinShare = 36;
 constexpr float kPtLift = 6.f;        // log2 of what weights are held times
 constexpr float kPtSlack = 8.f;       // log2 of how far the maximum in use may lag
@@ -154,14 +154,47 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
         "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-// Sixteen columns, waited for.
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+// Columns of this thread's row, waited for: the load and its wait are one, so that the registers
+// are not touched in between.
+__device__ __forceinline__ void tmem_ld16_now(uint32_t taddr, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
       "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
       "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld64_now(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+      "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, "
+      "%42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, "
+      "%62, %63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld32_now(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+      "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr)
       : "memory");
 }
@@ -179,15 +212,6 @@ __device__ __forceinline__ void tcgen05_mma_ts(uint32_t d_tmem, uint32_t a_tmem,
 // kind::f16 instruction descriptor: half x half -> f32, M 128, A K-major.
 __host__ __device__ constexpr uint32_t pt_idesc(int n, bool b_n_major) {
   return (1u << 4) | ((b_n_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-}
-// Waits for a tensor-memory load and names its registers, so that no use of them moves above.
-__device__ __forceinline__ void tmem_ld_wait32(uint32_t* r) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
-                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
-                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
-               ::"memory");
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -675,12 +699,9 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
         if (sub) ++n_tile;
         tcgen05_fence_after();
         uint32_t v[64];
-        tmem_ld32(col, v);
-        tmem_ld32(col + 32, v + 32);
+        tmem_ld64_now(col, v);
         // (key scale, log2 of the value scale, its inverse) of each 16 keys
         const uint4 f[4] = {pt_lds128(sc_at), pt_lds128(sc_at + 16), pt_lds128(sc_at + 32), pt_lds128(sc_at + 48)};
-        tmem_ld_wait32(v);
-        tmem_ld_wait32(v + 32);
         if (key0 < it.all_lo || key0 + 64 > it.all_hi) {
 #pragma unroll
           for (int k = 0; k < 64; ++k)
@@ -710,7 +731,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
 #pragma unroll 1
             for (int q = 0; q < D / 16; ++q) {
               uint32_t o[16];
-              tmem_ld16(o_col + q * 16, o);
+              tmem_ld16_now(o_col + q * 16, o);
 #pragma unroll
               for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * corr);
               tmem_st16(o_col + q * 16, o);
@@ -761,8 +782,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
       for (int q = 0; q < D / 32; ++q) {
         uint32_t v[32];
         __syncwarp();
-        tmem_ld32(o_col + q * 32, v);
-        tmem_ld_wait32(v);
+        tmem_ld32_now(o_col + q * 32, v);
         if (q == D / 32 - 1) {
           tcgen05_fence_before();
           mbar_arrive(o_free + i);     // the outputs are read: the next item's may come
