@@ -167,7 +167,8 @@ __global__ void __launch_bounds__(kStepThreads) page_step_kernel(
 
 // ---- rope_kv_pages --------------------------------------------------------------------------
 constexpr int kWriteThreads = 256;
-constexpr int kWriteRows = 8;      // rows a CTA looks at for the beginnings of page runs
+constexpr int kShortRun = 8;       // rows that one warp takes by itself
+constexpr int kHeld = 1;           // 16-element pieces a thread holds in registers: two cost more in occupancy (15.4 us for 13.4)
 
 struct WriteParams {
   const __nv_bfloat16* qkv;
@@ -180,6 +181,7 @@ struct WriteParams {
   const int* positions;
   int rows, H, G, S, log_page;
   long long slots_max;      // P * page
+  int chunk;                // rows a CTA of the k/v half looks at for the beginnings of page runs
   int kv_blocks;            // CTAs of the k/v half; the rest rotate q
 };
 
@@ -234,76 +236,82 @@ __device__ __forceinline__ uint32_t rescale_word(uint32_t w, float ratio) {
   return cvt_e4m3x2(lo.x * ratio, lo.y * ratio) | (cvt_e4m3x2(hi.x * ratio, hi.y * ratio) << 16);
 }
 
-// One run -- consecutive rows that go to consecutive slots of one page -- of one KV head, by the
-// `threads` threads that call this (a warp, or the CTA), `t` their index.  Every row takes
-// 2 * D / 16 threads: its key's, then its value's sixteen-element pieces.
+// One run -- consecutive rows that go to consecutive slots of one page -- of one KV head's keys or
+// values, by the `threads` threads that call this (a warp, or the CTA), `t` their index.  Every row
+// takes D / 16 threads, a sixteen-element piece each; up to kHeld pieces a thread stay in registers
+// between the maximum and the conversion, their loads all in flight at once; a longer run is read twice.
 template <int D, bool kBlock>
-__device__ __forceinline__ void write_run(const WriteParams& p, int row, int n, int slot, int g, int t, int threads,
-                                          float* red) {
-  constexpr int kPieces = D / 16, kPerRow = 2 * kPieces;
+__device__ __forceinline__ void write_run(const WriteParams& p, int row, int n, int slot, int g, int kind, int t,
+                                          int threads, float* red) {
+  constexpr int kPieces = D / 16;
   const int page = 1 << p.log_page, off = slot & (page - 1);
-  const long long pg = slot >> p.log_page;
-  float* sc = p.scales + (pg * p.G + g) * 2;
-  uint8_t* base = p.pool + (pg * p.G + g) * 2 * page * D;
-  const int piece = t % kPieces, kv = (t / kPieces) & 1, i0 = piece * 8;
-  const int head = p.H + kv * p.G + g;
-  const int rows_at_once = threads / kPerRow;
+  const long long at = ((long long)(slot >> p.log_page) * p.G + g) * 2 + kind;
+  uint8_t* base = p.pool + at * page * D;
+  const float old = off ? p.scales[at] : 0.f;
+  const int i0 = t % kPieces * 8, first = t / kPieces, rows_at_once = threads / kPieces;
+  const int head = p.H + kind * p.G + g;
+  const bool turn = kind == 0;
 
+  float ka[kHeld][8], kb[kHeld][8];
   float m = 0.f;
-  for (int i = t / kPerRow; i < n; i += rows_at_once) {
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) {
+    const int i = first + k * rows_at_once;
+    if (i < n) load_turned<D>(p, row + i, head, i0, turn, ka[k], kb[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+    if (first + k * rows_at_once < n) m = fmaxf(m, finite_amax(ka[k], kb[k]));
+  for (int i = first + kHeld * rows_at_once; i < n; i += rows_at_once) {
     float a[8], b[8];
-    load_turned<D>(p, row + i, head, i0, kv == 0, a, b);
+    load_turned<D>(p, row + i, head, i0, turn, a, b);
     m = fmaxf(m, finite_amax(a, b));
   }
-  // keys and values meet separately: lanes of one kind are kPieces wide, kPerRow apart
-#pragma unroll
-  for (int o = 1; o < kPieces; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-#pragma unroll
-  for (int o = kPerRow; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  float other = __shfl_xor_sync(0xffffffffu, m, kPieces);
-  float mk = kv ? other : m, mv = kv ? m : other;
+  m = warp_max(m);
   if (kBlock) {
-    const int warp = t >> 5;
-    if ((t & 31) == 0) { red[2 * warp] = mk; red[2 * warp + 1] = mv; }
+    if ((t & 31) == 0) red[t >> 5] = m;
     __syncthreads();
-    mk = red[0]; mv = red[1];
-    for (int w = 1; w < threads / 32; ++w) { mk = fmaxf(mk, red[2 * w]); mv = fmaxf(mv, red[2 * w + 1]); }
+    m = red[0];
+    for (int w = 1; w < threads / 32; ++w) m = fmaxf(m, red[w]);
   }
-  float old_k = 0.f, old_v = 0.f, sk = pow2_scale(mk), sv = pow2_scale(mv);
-  if (off) {   // the page goes on: it keeps the larger scale
-    old_k = sc[0]; old_v = sc[1];
-    sk = fmaxf(sk, old_k); sv = fmaxf(sv, old_v);
-  }
-  if (kBlock) __syncthreads(); else __syncwarp();   // the old scales have been read
-  if (t == 0) { sc[0] = sk; sc[1] = sv; }
-  if (off && (sk != old_k || sv != old_v)) {
-    // codes of earlier steps, 16 at a time; a ratio of powers of two is exact but for underflow
-    const int per = off * D / 16;
-    for (int i = t; i < 2 * per; i += threads) {
-      const bool v = i >= per;
-      const float ratio = v ? old_v / sv : old_k / sk;
-      if (ratio == 1.f) continue;
-      uint4* w = reinterpret_cast<uint4*>(base + (v ? (size_t)page * D : 0)) + (v ? i - per : i);
-      uint4 x = *w;
-      x.x = rescale_word(x.x, ratio); x.y = rescale_word(x.y, ratio);
-      x.z = rescale_word(x.z, ratio); x.w = rescale_word(x.w, ratio);
-      *w = x;
+  float scale = pow2_scale(m);
+  if (off) {
+    scale = fmaxf(scale, old);        // the page goes on: it keeps the larger scale
+    if (scale != old) {
+      // codes of earlier steps, 16 at a time; a ratio of powers of two is exact but for underflow
+      const float ratio = old / scale;
+      for (int i = t; i < off * kPieces; i += threads) {
+        uint4* w = reinterpret_cast<uint4*>(base) + i;
+        uint4 x = *w;
+        x.x = rescale_word(x.x, ratio); x.y = rescale_word(x.y, ratio);
+        x.z = rescale_word(x.z, ratio); x.w = rescale_word(x.w, ratio);
+        *w = x;
+      }
     }
   }
-  const float inv = 1.0f / (kv ? sv : sk);
-  for (int i = t / kPerRow; i < n; i += rows_at_once) {
+  if (kBlock) __syncthreads(); else __syncwarp();   // the old scale (and `red`) have been read
+  if (t == 0) p.scales[at] = scale;
+  const float inv = 1.0f / scale;
+  uint8_t* dst = base + (size_t)off * D + i0;
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) {
+    const int i = first + k * rows_at_once;
+    if (i < n) {
+      *reinterpret_cast<uint2*>(dst + (size_t)i * D) = e4m3_eight(ka[k], inv);
+      *reinterpret_cast<uint2*>(dst + (size_t)i * D + D / 2) = e4m3_eight(kb[k], inv);
+    }
+  }
+  for (int i = first + kHeld * rows_at_once; i < n; i += rows_at_once) {
     float a[8], b[8];
-    load_turned<D>(p, row + i, head, i0, kv == 0, a, b);
-    uint8_t* dst = base + ((size_t)kv * page + off + i) * D + i0;
-    *reinterpret_cast<uint2*>(dst) = e4m3_eight(a, inv);
-    *reinterpret_cast<uint2*>(dst + D / 2) = e4m3_eight(b, inv);
+    load_turned<D>(p, row + i, head, i0, turn, a, b);
+    *reinterpret_cast<uint2*>(dst + (size_t)i * D) = e4m3_eight(a, inv);
+    *reinterpret_cast<uint2*>(dst + (size_t)i * D + D / 2) = e4m3_eight(b, inv);
   }
 }
 
 template <int D>
-__global__ void __launch_bounds__(kWriteThreads) rope_kv_pages_kernel(const WriteParams p) {
-  __shared__ float red[2 * kWriteThreads / 32];
-  __shared__ int s_len;
+__global__ void __launch_bounds__(kWriteThreads, 4) rope_kv_pages_kernel(const WriteParams p) {
+  __shared__ float red[kWriteThreads / 32];
   pdl_wait();
   pdl_launch();
   const int tid = threadIdx.x;
@@ -322,40 +330,41 @@ __global__ void __launch_bounds__(kWriteThreads) rope_kv_pages_kernel(const Writ
     }
     return;
   }
-  // ---- k and v: a CTA looks at eight rows of one KV head for the beginnings of runs ----
-  const int g = blockIdx.x % p.G, r0 = blockIdx.x / p.G * kWriteRows;
+  // ---- k and v: a CTA looks at some rows (32 at most, a lane each) for the beginnings of runs and
+  // writes one KV head's keys or values of those ----
+  const int which = blockIdx.x % (2 * p.G), g = which % p.G, kind = which / p.G;
+  const int r0 = blockIdx.x / (2 * p.G) * p.chunk, r1 = min(r0 + p.chunk, p.rows);
   const int page = 1 << p.log_page, warp = tid >> 5, lane = tid & 31;
-  auto slot_of = [&](int r) { return r >= 0 && r < p.rows ? p.slots[r] : -1; };
-  auto begins = [&](int r) {
-    const int s = slot_of(r);
-    if (s < 0 || s >= p.slots_max) return false;
-    return (s & (page - 1)) == 0 || slot_of(r - 1) != s - 1;
+  auto slot_of = [&](int r) {
+    const int s = r >= 0 && r < p.rows ? p.slots[r] : -1;
+    return s < p.slots_max ? s : -1;
   };
-  // how many rows the run at r has, up to 33 as a warp sees them
-  auto run_of = [&](int r) {
-    const int s = slot_of(r), left = page - (s & (page - 1));
-    const bool on = lane < left && slot_of(r + lane) == s + lane;
-    const unsigned m = __ballot_sync(0xffffffffu, on);
-    return m == 0xffffffffu ? 33 : __ffs(~m) - 1;
-  };
-  // a short run is one warp's; a long one (more than eight rows) is the whole CTA's
-  const int mine = r0 + warp;
-  const bool here = mine < p.rows && begins(mine);
-  if (here) {
-    const int n = run_of(mine);
-    if (n <= kWriteRows) write_run<D, false>(p, mine, n, slot_of(mine), g, lane, 32, red);
-  }
-  for (int i = 0; i < kWriteRows; ++i) {
-    const int r = r0 + i;
-    if (r >= p.rows || !begins(r) || run_of(r) <= kWriteRows) continue;   // the same for every warp
-    const int s = slot_of(r), left = page - (s & (page - 1));
-    __syncthreads();
-    if (tid == 0) s_len = left;
-    __syncthreads();
-    for (int k = tid; k < left; k += kWriteThreads)
-      if (slot_of(r + k) != s + k) { atomicMin(&s_len, k); break; }
-    __syncthreads();
-    write_run<D, true>(p, r, s_len, s, g, tid, kWriteThreads, red);
+  const int mine = r0 + lane < r1 ? slot_of(r0 + lane) : -1, before = slot_of(r0 + lane - 1);
+  const bool goes_on = mine >= 0 && (mine & (page - 1)) != 0 && before == mine - 1;
+  const unsigned on = __ballot_sync(0xffffffffu, goes_on);
+  unsigned begin = __ballot_sync(0xffffffffu, mine >= 0 && !goes_on);
+  // a short run is one warp's, in turn; a longer one is the whole CTA's
+  for (int k = 0; begin; ++k) {
+    const int l = __ffs(begin) - 1;
+    begin &= begin - 1;
+    const int slot = __shfl_sync(0xffffffffu, mine, l), most = page - (slot & (page - 1));
+    int n = l == 31 ? 1 : __ffs(~(on >> (l + 1)));     // itself and the rows that go on
+    n = min(n, most);
+    if (r0 + l + n == r1 && n < most) {
+      // it may go on behind the rows looked at
+      for (bool more = true; more && n < most;) {
+        const bool same = n + lane < most && slot_of(r0 + l + n + lane) == slot + n + lane;
+        const unsigned m = __ballot_sync(0xffffffffu, same);
+        more = m == 0xffffffffu;
+        n += more ? 32 : __ffs(~m) - 1;
+      }
+    }
+    if (n <= kShortRun) {
+      if (k % (kWriteThreads / 32) == warp) write_run<D, false>(p, r0 + l, n, slot, g, kind, lane, 32, red);
+    } else {
+      __syncthreads();     // `red` is free
+      write_run<D, true>(p, r0 + l, n, slot, g, kind, tid, kWriteThreads, red);
+    }
   }
 }
 
@@ -410,7 +419,11 @@ extern "C" int iron_rope_kv_pages_e4m3(const void* qkv, long long pitch, const v
   if (rows < 0 || H <= 0 || G <= 0 || (D != 64 && D != 128) || S <= 0 || P <= 0 || log_page < 0) return IRON_ERR_SHAPE;
   if ((long long)P * page_size > 0x7fffffffll) return IRON_ERR_SHAPE;
   if (pitch < (long long)(H + 2 * G) * D || (pitch & 7)) return IRON_ERR_SHAPE;
-  const long long kv_blocks = ((long long)rows + kWriteRows - 1) / kWriteRows * G;
+  // Rows a CTA looks at: a decode batch's rows are runs of one, a warp each, and want many CTAs; a
+  // prompt's are runs of a page, and a CTA that finds none is in the way (2048 rows of a prompt, 32
+  // heads over 8 of 128, pages of 64: 13.4 us with 32, 18.1 with 8; 64 single rows: 6.2 us with 8).
+  const int chunk = rows > 1024 ? 32 : kShortRun;
+  const long long kv_blocks = ((long long)rows + chunk - 1) / chunk * 2 * G;
   if (kv_blocks > 0x3fffffffll) return IRON_ERR_SHAPE;
   if (rows == 0) return IRON_OK;
   if (!qkv || !angles || !q_out || !pool || !scales || !slots || !positions) return IRON_ERR_SHAPE;
@@ -420,6 +433,7 @@ extern "C" int iron_rope_kv_pages_e4m3(const void* qkv, long long pitch, const v
   p.q_out = (__nv_bfloat16*)q_out; p.pool = (uint8_t*)pool; p.scales = scales; p.slots = slots;
   p.positions = positions; p.rows = rows; p.H = H; p.G = G; p.S = S; p.log_page = log_page;
   p.slots_max = (long long)P * page_size;
+  p.chunk = chunk;
   p.kv_blocks = (int)kv_blocks;
   const long long q_items = (long long)rows * H * (D / 16);
   long long q_blocks = (q_items + kWriteThreads - 1) / kWriteThreads;

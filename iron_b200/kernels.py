@@ -578,13 +578,13 @@ def _on_device(*ts) -> int:
     These calls are a few microseconds of work on the device, so the checks are kept as cheap."""
     dev = ts[0].get_device()
     for t in ts:
-        if t.get_device() != dev or dev < 0 or not t.is_contiguous():
+        if t.get_device() != dev or not t.is_contiguous() or dev < 0:
             if not t.is_cuda:
                 raise RuntimeError("iron_b200 kernels take CUDA tensors only (no CPU fallback)")
             if not t.is_contiguous():
                 raise ValueError("iron_b200 kernels take contiguous tensors")
             raise ValueError(f"a tensor of cuda:{t.get_device()} in a call on cuda:{dev}")
-    if dev != torch.cuda.current_device():
+    if dev != torch._C._cuda_getDevice():
         raise ValueError(f"tensors of cuda:{dev} in a call on cuda:{torch.cuda.current_device()}")
     return torch._C._cuda_getCurrentRawStream(dev)
 
@@ -619,26 +619,30 @@ def page_step(tables, lengths, new_tokens, pages, ring, *, page_size, rows, leng
     if tables.dim() != 2 or lengths.dim() != 1 or new_tokens.shape != lengths.shape or tables.shape[0] != lengths.shape[0]:
         raise ValueError(f"tables {tuple(tables.shape)}, lengths {tuple(lengths.shape)} and new_tokens "
                          f"{tuple(new_tokens.shape)} are not (B, width), (B,) and (B,)")
-    if pages.dim() != 1 or ring.shape != (4,):
+    if pages.dim() != 1 or ring.dim() != 1 or ring.numel() != 4:
         raise ValueError(f"pages {tuple(pages.shape)} and ring {tuple(ring.shape)} are not (P,) and (4,)")
     B, width = tables.shape
     if rows < 0:
         raise ValueError(f"rows ({rows}) is negative")
-    outs = (slots, positions, row_start, lengths_out, ring_out)
-    sizes = (rows, rows, B + 1, B, 4)
-    if any(t is None for t in outs):   # one allocation for all that are missing
-        made = torch.empty(2 * B + 2 * rows + 5, dtype=torch.int32, device=tables.device).split(sizes)
-        outs = tuple(m if t is None else t for t, m in zip(outs, made))
-    for t, n in zip(outs, sizes):
-        if t.dim() != 1 or t.shape[0] != n:
-            raise ValueError("outputs are slots (rows,), positions (rows,), row_start (B + 1,), lengths_out (B,), ring_out (4,)")
-    _int32("page_step's tensors", tables, lengths, new_tokens, pages, ring, *outs)
-    stream = _on_device(tables, lengths, new_tokens, pages, ring, *outs)
-    slots, positions, row_start, lengths_out, ring_out = outs
+    if slots is None or positions is None or row_start is None or lengths_out is None or ring_out is None:
+        # one allocation for all that are missing
+        made = torch.empty(2 * (B + rows) + 5, dtype=torch.int32, device=tables.device)
+        made = torch.split_with_sizes(made, (rows, rows, B + 1, B, 4))
+        slots = made[0] if slots is None else slots
+        positions = made[1] if positions is None else positions
+        row_start = made[2] if row_start is None else row_start
+        lengths_out = made[3] if lengths_out is None else lengths_out
+        ring_out = made[4] if ring_out is None else ring_out
+    if not (slots.dim() == positions.dim() == row_start.dim() == lengths_out.dim() == ring_out.dim() == 1
+            and slots.numel() == positions.numel() == rows and row_start.numel() == B + 1
+            and lengths_out.numel() == B and ring_out.numel() == 4):
+        raise ValueError("outputs are slots (rows,), positions (rows,), row_start (B + 1,), lengths_out (B,), ring_out (4,)")
+    _int32("page_step's tensors", tables, lengths, new_tokens, pages, ring, slots, positions, row_start, lengths_out, ring_out)
+    stream = _on_device(tables, lengths, new_tokens, pages, ring, slots, positions, row_start, lengths_out, ring_out)
     call("iron_page_step", tables.data_ptr(), width, lengths.data_ptr(), new_tokens.data_ptr(), B, pages.data_ptr(),
-         pages.shape[0], ring.data_ptr(), int(page_size), int(rows), lengths_out.data_ptr(), ring_out.data_ptr(),
+         pages.numel(), ring.data_ptr(), page_size, rows, lengths_out.data_ptr(), ring_out.data_ptr(),
          slots.data_ptr(), positions.data_ptr(), row_start.data_ptr(), stream)
-    return outs
+    return slots, positions, row_start, lengths_out, ring_out
 
 
 def rope_kv_pages(qkv, angles, q_out, pool, scales, slots, positions, *, H, G, D):
