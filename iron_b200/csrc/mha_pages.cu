@@ -1,5 +1,5 @@
-// Attention over a key/value cache that lies in pages of e4m3 codes, on warp MMAs: one query a
-// sequence (a decode step), or the few rows a sequence brings (a draft to verify, a short chunk).
+// Attention of one query a sequence (a decode step) over a key/value cache that lies in pages of
+// e4m3 codes, on warp MMAs; and the C entries of this and of the ragged form (mha_pages_tc.cu).
 //
 // Bound by the cache's bytes, so the kernel is built around keeping them coming: every warp has
 // a ring of its own in shared memory that TMA fills (16 tokens of one page and head a box, the
@@ -28,6 +28,8 @@
 // segments, end to end, are cut into equal runs, one a CTA, so ragged lengths leave no CTA idle.
 // A CTA's four warps take a run's units in turn and merge in shared memory; a segment cut by a CTA
 // boundary leaves partials in the workspace, which a second small launch folds in order.
+#include <type_traits>
+
 #include "common.cuh"
 #include "mma.cuh"
 #include "pages.cuh"
@@ -37,34 +39,25 @@ namespace iron {
 
 constexpr int kPgWarps = 4;
 constexpr int kPgThreads = kPgWarps * 32;
-constexpr int kPgCtasPerSm = 3;
-constexpr int kPgCtas = kSMs * kPgCtasPerSm;
+// CTAs an SM: what the registers of one or of two groups of eight columns allow without spilling
+constexpr int pg_ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+constexpr int kPgCtas = kSMs * pg_ctas_per_sm(1);
 constexpr int kPgUnit = 16;                 // tokens
 constexpr int kPgStages = 2;                // of a warp's ring; a stage holds kGroup units
-constexpr int kPgSegCost = 16;              // units a segment costs beside its own (queries, merge)
+constexpr int kPgSegCost = 24;              // units a segment costs beside its own (queries, merge)
 constexpr float kPgLift = 10.f;             // log2 of what probabilities are held times
 
-// A sequence as the kernels see it: its keys, its query rows, and the units a segment spans.
+// A sequence as the kernel sees it: its keys [lo, len), the first unit of 16 that holds one, and how
+// many units a segment -- a KV head's group of columns -- has.  An empty one still has a unit:
+// somebody must write its zeros.
 struct PagesSeq {
-  int len, row0, n, unit0;      // keys, first row, rows, first unit any row may see
-  int blocks;                   // column blocks: G times as many segments
-  int units;                    // units of a segment
+  int len, lo, unit0, units;
 };
-
-template <int COLS>
 __device__ __forceinline__ PagesSeq pages_seq(const PagesParams& p, int b) {
   PagesSeq s;
   s.len = max(0, (int)min((long long)p.lengths[b], (long long)p.width << p.log_page));
-  if (p.row_start) {
-    s.row0 = min(max(p.row_start[b], 0), p.rows);
-    s.n = max(0, min(p.row_start[b + 1], p.rows) - s.row0);
-  } else {
-    s.row0 = b; s.n = 1;
-  }
-  const int first = p.window >= 0 ? max(0, s.len - s.n - p.window) : 0;
-  s.unit0 = first / kPgUnit;
-  s.blocks = (s.n * p.hg + COLS - 1) / COLS;
-  // an empty segment still has a unit: somebody must write its zeros
+  s.lo = p.window >= 0 ? max(0, s.len - 1 - p.window) : 0;
+  s.unit0 = s.lo / kPgUnit;
   s.units = max(1, (s.len + kPgUnit - 1) / kPgUnit - s.unit0);
   return s;
 }
@@ -83,9 +76,9 @@ struct PgCfg {
   static constexpr int kSmem = kBars + 128 + 1024;
 };
 
-// what a sequence's segments cost in units
-__device__ __forceinline__ long long pages_cost(const PagesParams& p, const PagesSeq& s) {
-  return (long long)p.G * s.blocks * (s.units + kPgSegCost);
+// what a sequence's segments cost in units; `segs`: KV heads times groups of columns
+__device__ __forceinline__ long long pages_cost(int segs, const PagesSeq& s) {
+  return (long long)segs * (s.units + kPgSegCost);
 }
 
 // units per CTA: an equal share, and two groups a warp at least
@@ -129,14 +122,14 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
 
 // One segment's piece of a CTA's share.
 struct PagesPiece {
-  int b, gh, col0, cols;        // sequence, KV head, first query column, columns
-  int u_lo, u_hi;               // units of the segment
-  int first, last;              // units some column sees, within [u_lo, u_hi)
-  long long seg_at;             // where the segment begins in the dealt-out units
+  int b, gh, col0, cols;        // sequence, KV head, first query head of its group, heads
+  PagesSeq seq;
+  int first, last;              // units of the segment
+  long long end_at;             // where the segment ends in the dealt-out units
 };
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kPgThreads, kPgCtasPerSm)
+__global__ void __launch_bounds__(kPgThreads, pg_ctas_per_sm(NT))
 mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
   using Cfg = PgCfg<D, NT>;
   constexpr int COLS = Cfg::kCols, U = Cfg::kGroup;
@@ -150,6 +143,7 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pg_smem_raw) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int hg = p.hg, page_mask = (1 << p.log_page) - 1;
+  const int blocks = (hg + COLS - 1) / COLS, segs = p.G * blocks;
   float* s_o = reinterpret_cast<float*>(smem + Cfg::kMerge);   // [warp][column][D / kParts]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kBars) + warp * kPgStages;
   const uint32_t ring = smem_u32(smem + Cfg::kRing) + warp * kPgStages * Cfg::kStage;
@@ -169,8 +163,8 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
   const int sb = min(tid * per_thread, p.B), se = min(sb + per_thread, p.B);
   long long mine = 0;
   for (int b = sb; b < se; ++b) {
-    const PagesSeq s = pages_seq<COLS>(p, b);
-    mine += pages_cost(p, s);
+    const PagesSeq s = pages_seq(p, b);
+    mine += pages_cost(segs, s);
   }
   long long before = mine, total = 0;
 #pragma unroll
@@ -193,8 +187,8 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
   if (begin >= before && begin < before + mine) {
     long long acc = before;
     for (int b = sb; b < se; ++b) {
-      const PagesSeq s = pages_seq<COLS>(p, b);
-      const long long w = pages_cost(p, s);
+      const PagesSeq s = pages_seq(p, b);
+      const long long w = pages_cost(segs, s);
       if (begin < acc + w) { s_b = b; s_at = acc; break; }
       acc += w;
     }
@@ -203,34 +197,30 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
   volatile int* abort_flag = &s_abort;
   int seq_b = s_b;
   long long seq_at = s_at;      // where sequence seq_b begins in the dealt-out units
-  PagesSeq seq = pages_seq<COLS>(p, seq_b);
+  PagesSeq seq = pages_seq(p, seq_b);
 
   // The piece of the share [at, end) that begins at `at`; false when nothing is left.  A segment's
   // units follow the kPgSegCost that it costs beside them, so a share may hold none of its own.
   auto next_piece = [&](long long& at, PagesPiece& x) {
     while (at < end) {
-      for (long long w; at >= seq_at + (w = pages_cost(p, seq));) {
+      for (long long w; at >= seq_at + (w = pages_cost(segs, seq));) {
         seq_at += w;
-        seq = pages_seq<COLS>(p, ++seq_b);
+        seq = pages_seq(p, ++seq_b);
       }
       const int span = seq.units + kPgSegCost;
       const int seg = (int)div_ll(at - seq_at, span);
-      x.seg_at = seq_at + (long long)seg * span;
-      const int lo = (int)(at - x.seg_at), hi = (int)(min(end, x.seg_at + span) - x.seg_at);
-      at = x.seg_at + hi;
-      x.u_lo = max(lo - kPgSegCost, 0);
-      x.u_hi = max(hi - kPgSegCost, 0);
-      if (x.u_lo >= x.u_hi) continue;
+      const long long seg_at = seq_at + (long long)seg * span;
+      const int lo = (int)(at - seg_at), hi = (int)(min(end, seg_at + span) - seg_at);
+      at = seg_at + hi;
+      x.first = max(lo - kPgSegCost, 0);
+      x.last = max(hi - kPgSegCost, 0);
+      if (x.first >= x.last) continue;
       x.b = seq_b;
-      x.gh = seq.blocks == 1 ? seg : seg / seq.blocks;
-      x.col0 = (seg - x.gh * seq.blocks) * COLS;
-      x.cols = min(COLS, seq.n * hg - x.col0);
-      int any_lo = 0, any_hi = seq.len;
-      const int past = seq.len - seq.n;
-      if (p.causal) any_hi = min(any_hi, past + (x.col0 + x.cols - 1) / hg + 1);
-      if (p.window >= 0) any_lo = max(0, past + x.col0 / hg - p.window);
-      x.first = max(x.u_lo, any_lo / kPgUnit - seq.unit0);
-      x.last = min(x.u_hi, (max(any_hi, 0) + kPgUnit - 1) / kPgUnit - seq.unit0);
+      x.gh = blocks == 1 ? seg : seg / blocks;
+      x.col0 = (seg - x.gh * blocks) * COLS;
+      x.cols = min(COLS, hg - x.col0);
+      x.seq = seq;
+      x.end_at = seg_at + span;
       return true;
     }
     return false;
@@ -239,10 +229,11 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
   int filled = 0, drained = 0;   // groups of this warp so far: a group's stage and phase
   // lane l looks up unit l % U of group l / U of a batch of NB groups
   struct Batch { int entry; float sk, log_v, inv_v; };
-  auto look_up = [&](const PagesPiece& x, int unit0, int k0) {
+  auto look_up = [&](const PagesPiece& x, int k0) {
     const int u = x.first + ((k0 + lane / U) * kPgWarps + warp) * U + lane % U;
     int e = -1;
-    if (u < x.last) e = p.tables[(long long)x.b * p.width + min(((unit0 + u) * kPgUnit) >> p.log_page, p.width - 1)];
+    if (u < x.last && x.seq.len > 0)
+      e = p.tables[(long long)x.b * p.width + (((x.seq.unit0 + u) * kPgUnit) >> p.log_page)];
     return e >= 0 && e < p.P ? e : -1;
   };
   auto look_up_scales = [&](const PagesPiece& x, Batch& q) {
@@ -253,7 +244,7 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
     q.inv_v = 1.f / s.y;
   };
   // group k of the piece into the ring: lanes 0 .. U - 1 a unit each
-  auto fill = [&](const PagesPiece& x, int unit0, const Batch& q, int k) {
+  auto fill = [&](const PagesPiece& x, const Batch& q, int k) {
     const int entry = __shfl_sync(0xffffffffu, q.entry, (k % NB) * U + (lane % U));
     const int u = x.first + (k * kPgWarps + warp) * U + lane;
     const bool on = lane < U && entry >= 0;
@@ -263,53 +254,44 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
     __syncwarp();
     if (on) {
       const uint32_t dst = ring + stage * Cfg::kStage + lane * 2 * Cfg::kHalf, bar = smem_u32(bars + stage);
-      const int off = ((unit0 + u) * kPgUnit) & page_mask, block = entry * p.G + x.gh;
+      const int off = ((x.seq.unit0 + u) * kPgUnit) & page_mask, block = entry * p.G + x.gh;
       tma_load_3d(dst, &map, 0, off, block, bar);
       tma_load_3d(dst + Cfg::kHalf, &map, 0, page_mask + 1 + off, block, bar);
     }
     ++filled;
   };
   auto groups_of = [&](const PagesPiece& x) {
-    const int units = x.last - x.first, groups = (max(units, 0) + U - 1) / U;
+    const int groups = (x.last - x.first + U - 1) / U;
     return (groups - warp + kPgWarps - 1) / kPgWarps;
   };
 
   long long at = begin;
   PagesPiece cur;
-  PagesSeq cur_seq = seq;
   Batch bat, bat_next;
-  uint4 q_raw[NT][D / 32];      // this lane's share of the queries of columns 8 nt + g: a run of D / 4
+  uint4 q_raw[NT][D / 32];      // this lane's share of the query of column 8 nt + g: a run of D / 4
   // the loads that a piece begins with, in the order in which others wait for them
   auto open_piece = [&]() {
-    bat.entry = look_up(cur, cur_seq.unit0, 0);
-    bat_next.entry = look_up(cur, cur_seq.unit0, NB);
+    bat.entry = look_up(cur, 0);
+    bat_next.entry = look_up(cur, NB);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int c = nt * 8 + g;
-      const bool live = c < cur.cols;
-      const int row = live ? (cur.col0 + c) / hg : 0, h = live ? (cur.col0 + c) - row * hg : 0;
-      const __nv_bfloat16* src = p.q + ((long long)(cur_seq.row0 + row) * p.H + cur.gh * hg + h) * D + t * (D / 4);
+      const __nv_bfloat16* src = p.q + ((long long)cur.b * p.H + cur.gh * hg + cur.col0 + c) * D + t * (D / 4);
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) q_raw[nt][i] = live ? ld_cached(src + 8 * i) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < D / 32; ++i) q_raw[nt][i] = c < cur.cols ? ld_cached(src + 8 * i) : make_uint4(0, 0, 0, 0);
     }
     const int n = groups_of(cur);
-    for (int k = 0; k < kPgStages && k < n; ++k) fill(cur, cur_seq.unit0, bat, k);
+    for (int k = 0; k < kPgStages && k < n; ++k) fill(cur, bat, k);
     look_up_scales(cur, bat);
     look_up_scales(cur, bat_next);
   };
   bool have = next_piece(at, cur);
-  cur_seq = seq;
   bool ok = true;
-  if (have) {
-    open_piece();
-  }
+  if (have) open_piece();
   while (have) {
-    const int past = cur_seq.len - cur_seq.n;     // position of the first row
-    const int len = cur_seq.len, unit0 = cur_seq.unit0;
     // ---- Q: this lane's share of column 8 nt + g, in halves under a power of two ----
     uint32_t qf[NT][KS][2];
     float colfac[NT][2];                        // of columns 8 nt + 2t and + 1
-    int hi_key[NT][2], lo_key[NT][2];           // keys those columns see: [lo, hi)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float mx = 0.f;
@@ -337,17 +319,8 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
         }
       }
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        colfac[nt][j] = __shfl_sync(0xffffffffu, down, (2 * t + j) * 4) * p.scale_log2;
-        const int cc = nt * 8 + 2 * t + j;
-        const int pos = past + (cur.col0 + min(cc, cur.cols - 1)) / hg;
-        hi_key[nt][j] = cc < cur.cols ? (p.causal ? min(len, pos + 1) : len) : 0;
-        lo_key[nt][j] = p.window >= 0 ? pos - p.window : 0;
-      }
+      for (int j = 0; j < 2; ++j) colfac[nt][j] = __shfl_sync(0xffffffffu, down, (2 * t + j) * 4) * p.scale_log2;
     }
-    // the keys that every column sees
-    const int all_hi = p.causal ? min(len, past + cur.col0 / hg + 1) : len;
-    const int all_lo = p.window >= 0 ? past + (cur.col0 + cur.cols - 1) / hg - p.window : 0;
 
     float o[KS][NT][4], m_run[NT][2], l_run[NT][2];
 #pragma unroll
@@ -368,184 +341,151 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
       if (!ok) break;
       ++drained;
       const uint32_t base = ring + stage * Cfg::kStage;
-      const int src0 = (k % NB) * U;
-      // ---- S^T = K Q^T ----
-      float s[U][NT][4];
-      bool whole[U], present[U];
+      const int src0 = (k % NB) * U, tok0 = (cur.seq.unit0 + cur.first + (k * kPgWarps + warp) * U) * kPgUnit;
+      // Whether every unit of the group is there and its tokens are all keys.  The common case goes
+      // without a branch, so that the units' chains of products interleave.
+      const bool whole = __all_sync(0xffffffffu, __shfl_sync(0xffffffffu, bat.entry, src0 + lane % U) >= 0) &&
+                         tok0 >= cur.seq.lo && tok0 + U * kPgUnit <= cur.seq.len;
+      auto key = [&](int tok) { return tok >= cur.seq.lo && tok < cur.seq.len; };
+      auto group = [&](auto is_whole) {
+        constexpr bool kWhole = decltype(is_whole)::value;
+        // ---- S^T = K Q^T ----
+        float s[U][NT][4];
+        uint32_t kf[U][2][D / 16];
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        present[i] = __shfl_sync(0xffffffffu, bat.entry, src0 + i) >= 0;
-        const float sk = __shfl_sync(0xffffffffu, bat.sk, src0 + i), lv = __shfl_sync(0xffffffffu, bat.log_v, src0 + i);
-        const int tok0 = (unit0 + cur.first + (k * kPgWarps + warp) * U + i) * kPgUnit;
-        whole[i] = present[i] && tok0 + kPgUnit <= all_hi && tok0 >= all_lo;
-        uint32_t kf[2][D / 16];
-        const uint32_t kb = base + i * 2 * Cfg::kHalf;
+        for (int i = 0; i < U; ++i) {
+          const uint32_t kb = base + i * 2 * Cfg::kHalf;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          if (D == 128) {
-            const uint32_t row = kb + (g + 8 * r) * 128;
-            const uint4 x = lds128(row + (((2 * t) ^ g) << 4)), y = lds128(row + (((2 * t + 1) ^ g) << 4));
-            kf[r][0] = x.x; kf[r][1] = x.y; kf[r][2] = x.z; kf[r][3] = x.w;
-            kf[r][D / 16 - 4] = y.x; kf[r][D / 16 - 3] = y.y; kf[r][D / 16 - 2] = y.z; kf[r][D / 16 - 1] = y.w;
-          } else {
-            const uint4 x = lds128(kb + (g + 8 * r) * 64 + ((t ^ ((g >> 1) & 3)) << 4));
-            kf[r][0] = x.x; kf[r][1] = x.y; kf[r][2] = x.z; kf[r][3] = x.w;
+          for (int r = 0; r < 2; ++r) {
+            if (D == 128) {
+              const uint32_t row = kb + (g + 8 * r) * 128;
+              const uint4 x = lds128(row + (((2 * t) ^ g) << 4)), y = lds128(row + (((2 * t + 1) ^ g) << 4));
+              kf[i][r][0] = x.x; kf[i][r][1] = x.y; kf[i][r][2] = x.z; kf[i][r][3] = x.w;
+              kf[i][r][D / 16 - 4] = y.x; kf[i][r][D / 16 - 3] = y.y; kf[i][r][D / 16 - 2] = y.z; kf[i][r][D / 16 - 1] = y.w;
+            } else {
+              const uint4 x = lds128(kb + (g + 8 * r) * 64 + ((t ^ ((g >> 1) & 3)) << 4));
+              kf[i][r][0] = x.x; kf[i][r][1] = x.y; kf[i][r][2] = x.z; kf[i][r][3] = x.w;
+            }
           }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) s[i][nt][0] = s[i][nt][1] = s[i][nt][2] = s[i][nt][3] = 0.f;
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) s[i][nt][0] = s[i][nt][1] = s[i][nt][2] = s[i][nt][3] = 0.f;
+        for (int c = 0; c < KS; ++c)
 #pragma unroll
-        for (int c = 0; c < KS; ++c) {
-          const uint32_t a[4] = {e4m3x2_to_half2(kf[0][c]), e4m3x2_to_half2(kf[1][c]),
-                                 e4m3x2_to_half2(kf[0][c] >> 16), e4m3x2_to_half2(kf[1][c] >> 16)};
+          for (int i = 0; i < U; ++i) {
+            const uint32_t a[4] = {e4m3x2_to_half2(kf[i][0][c]), e4m3x2_to_half2(kf[i][1][c]),
+                                   e4m3x2_to_half2(kf[i][0][c] >> 16), e4m3x2_to_half2(kf[i][1][c] >> 16)};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_f16_16816(s[i][nt], a, qf[nt][c][0], qf[nt][c][1]);
-        }
+            for (int nt = 0; nt < NT; ++nt) mma_f16_16816(s[i][nt], a, qf[nt][c][0], qf[nt][c][1]);
+          }
+        // ---- scales, running maximum ----
+        float m_new[NT][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) m_new[nt][0] = m_run[nt][0], m_new[nt][1] = m_run[nt][1];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[i][nt][j] = fmaf(s[i][nt][j], colfac[nt][j & 1] * sk, lv);
-        if (!whole[i]) {
+        for (int i = 0; i < U; ++i) {
+          const float sk = __shfl_sync(0xffffffffu, bat.sk, src0 + i), lv = __shfl_sync(0xffffffffu, bat.log_v, src0 + i);
+          bool seen[2] = {true, true};
+          if (!kWhole) {
+            const bool there = __shfl_sync(0xffffffffu, bat.entry, src0 + i) >= 0;
+            seen[0] = there && key(tok0 + i * kPgUnit + g);
+            seen[1] = there && key(tok0 + i * kPgUnit + g + 8);
+          }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const int key = tok0 + g + (j >> 1) * 8;
-              if (!present[i] || key >= hi_key[nt][j & 1] || key < lo_key[nt][j & 1]) s[i][nt][j] = -INFINITY;
+              s[i][nt][j] = seen[j >> 1] ? fmaf(s[i][nt][j], colfac[nt][j & 1] * sk, lv) : -INFINITY;
+              m_new[nt][j & 1] = fmaxf(m_new[nt][j & 1], s[i][nt][j]);
             }
         }
-      }
-      // ---- running maximum and sum ----
-      float m_new[NT][2];
-      bool moved = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float m = fmaxf(s[0][nt][j], s[0][nt][j + 2]);
-#pragma unroll
-          for (int i = 1; i < U; ++i) m = fmaxf(m, fmaxf(s[i][nt][j], s[i][nt][j + 2]));
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-          m_new[nt][j] = fmaxf(m_run[nt][j], m);
-          moved = moved || m_new[nt][j] != m_run[nt][j];
-        }
-      if (__any_sync(0xffffffffu, moved)) {   // seldom after the first groups
+        bool moved = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float corr = ex2(m_run[nt][j] - (m_new[nt][j] == -INFINITY ? 0.f : m_new[nt][j]));
-            m_run[nt][j] = m_new[nt][j];
-            l_run[nt][j] *= corr;
-#pragma unroll
-            for (int i = 0; i < KS; ++i) { o[i][nt][j] *= corr; o[i][nt][j + 2] *= corr; }
+            float& m = m_new[nt][j];
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+            moved = moved || m != m_run[nt][j];
           }
-      }
+        if (__any_sync(0xffffffffu, moved)) {   // seldom after the first groups
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        if (!present[i]) continue;              // the stage holds nothing there
-        const float inv_v = __shfl_sync(0xffffffffu, bat.inv_v, src0 + i);
-        uint32_t pb[NT][2];
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float pr[4];
+            for (int j = 0; j < 2; ++j) {
+              const float corr = ex2(m_run[nt][j] - (m_new[nt][j] == -INFINITY ? 0.f : m_new[nt][j]));
+              m_run[nt][j] = m_new[nt][j];
+              l_run[nt][j] *= corr;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float zero = (m_run[nt][j] == -INFINITY ? 0.f : m_run[nt][j]) - kPgLift;
-            pr[j] = ex2(s[i][nt][j] - zero);
-            pr[j + 2] = ex2(s[i][nt][j + 2] - zero);
-            l_run[nt][j] = fmaf(pr[j] + pr[j + 2], inv_v, l_run[nt][j]);
-          }
-          pb[nt][0] = movmatrix_trans(pack_half2(pr[0], pr[1]));
-          pb[nt][1] = movmatrix_trans(pack_half2(pr[2], pr[3]));
-        }
-        uint32_t vf[4][D / 32];
-        const uint32_t vb = base + i * 2 * Cfg::kHalf + Cfg::kHalf;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = 2 * t + (r & 1) + (r >> 1) * 8;
-          if (D == 128) {
-            const uint4 x = lds128(vb + row * 128 + ((g ^ (row & 7)) << 4));
-            vf[r][0] = x.x; vf[r][1] = x.y; vf[r][D / 32 - 2] = x.z; vf[r][D / 32 - 1] = x.w;
-          } else {
-            const uint2 x = lds64(vb + row * 64 + ((((g >> 1) ^ ((row >> 1) & 3)) << 4) | ((g & 1) << 3)));
-            vf[r][0] = x.x; vf[r][1] = x.y;
-          }
-        }
-        // ---- a NaN value of a token some column does not see must not reach it through 0 x NaN ----
-        if (!whole[i]) {
-          uint32_t bad = 0;
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int w = 0; w < D / 32; ++w) bad |= nan_codes(vf[r][w]);
-          if (__any_sync(0xffffffffu, bad != 0)) {
-            // NaN codes become zeros; where a column sees one, its output becomes NaN: the counts
-            // of (NaN, seen) pairs are a product of the same shape
-            const int tok0 = (unit0 + cur.first + (k * kPgWarps + warp) * U + i) * kPgUnit;
-            uint32_t seen[NT][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int key = tok0 + g + h * 8;
-                const bool s0 = key < hi_key[nt][0] && key >= lo_key[nt][0];
-                const bool s1 = key < hi_key[nt][1] && key >= lo_key[nt][1];
-                seen[nt][h] = movmatrix_trans((s0 ? 0x3c00u : 0u) | (s1 ? 0x3c000000u : 0u));
-              }
-#pragma unroll
-            for (int c = 0; c < KS; ++c) {
-              const int w = c >> 1, sh = 16 * (c & 1);
-              uint32_t a[4];
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {      // a0: byte 0 of tokens 0, 1; a1: byte 1; a2, a3: tokens 2, 3
-                const uint32_t x = nan_codes(vf[(r >> 1) * 2][w]) >> (sh + 8 * (r & 1) + 7);
-                const uint32_t y = nan_codes(vf[(r >> 1) * 2 + 1][w]) >> (sh + 8 * (r & 1) + 7);
-                a[r] = ((x & 1u) ? 0x3c00u : 0u) | ((y & 1u) ? 0x3c000000u : 0u);
-              }
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                float n[4] = {0.f, 0.f, 0.f, 0.f};
-                mma_f16_16816(n, a, seen[nt][0], seen[nt][1]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  if (n[j] > 0.f) o[c][nt][j] = __uint_as_float(0x7fc00000u);
-              }
+              for (int c = 0; c < KS; ++c) { o[c][nt][j] *= corr; o[c][nt][j + 2] *= corr; }
             }
+        }
+        // ---- weights and their sum; O^T += V^T P^T ----
+        float zero[NT][2];
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int w = 0; w < D / 32; ++w) vf[r][w] &= ~((nan_codes(vf[r][w]) >> 7) * 0xffu);
+          for (int j = 0; j < 2; ++j) zero[nt][j] = (m_run[nt][j] == -INFINITY ? 0.f : m_run[nt][j]) - kPgLift;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          const float inv_v = __shfl_sync(0xffffffffu, bat.inv_v, src0 + i);
+          uint32_t pb[NT][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float pr[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) pr[j] = ex2(s[i][nt][j] - zero[nt][j & 1]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) l_run[nt][j] = fmaf(pr[j] + pr[j + 2], inv_v, l_run[nt][j]);
+            pb[nt][0] = movmatrix_trans(pack_half2(pr[0], pr[1]));
+            pb[nt][1] = movmatrix_trans(pack_half2(pr[2], pr[3]));
+          }
+          uint32_t vf[4][D / 32];
+          const uint32_t vb = base + i * 2 * Cfg::kHalf + Cfg::kHalf;
+          const bool there = kWhole || __shfl_sync(0xffffffffu, bat.entry, src0 + i) >= 0;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int row = 2 * t + (r & 1) + (r >> 1) * 8;
+            if (D == 128) {
+              const uint4 x = lds128(vb + row * 128 + ((g ^ (row & 7)) << 4));
+              vf[r][0] = x.x; vf[r][1] = x.y; vf[r][D / 32 - 2] = x.z; vf[r][D / 32 - 1] = x.w;
+            } else {
+              const uint2 x = lds64(vb + row * 64 + ((((g >> 1) ^ ((row >> 1) & 3)) << 4) | ((g & 1) << 3)));
+              vf[r][0] = x.x; vf[r][1] = x.y;
+            }
+            // what lies where no key does (a page's tail, an absent page) may be NaN, and 0 x NaN is NaN
+            if (!kWhole && !(there && key(tok0 + i * kPgUnit + row)))
+#pragma unroll
+              for (int w = 0; w < D / 32; ++w) vf[r][w] = 0;
+          }
+#pragma unroll
+          for (int c = 0; c < KS; ++c) {
+            const uint32_t sel = (c & 1) ? 0x7362u : 0x5140u;
+            const uint32_t x = prmt(vf[0][c >> 1], vf[1][c >> 1], sel), y = prmt(vf[2][c >> 1], vf[3][c >> 1], sel);
+            const uint32_t a[4] = {e4m3x2_to_half2(x), e4m3x2_to_half2(x >> 16), e4m3x2_to_half2(y), e4m3x2_to_half2(y >> 16)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_f16_16816(o[c][nt], a, pb[nt][0], pb[nt][1]);
           }
         }
-        // ---- O^T += V^T P^T ----
-#pragma unroll
-        for (int c = 0; c < KS; ++c) {
-          const uint32_t sel = (c & 1) ? 0x7362u : 0x5140u;
-          const uint32_t x = prmt(vf[0][c >> 1], vf[1][c >> 1], sel), y = prmt(vf[2][c >> 1], vf[3][c >> 1], sel);
-          const uint32_t a[4] = {e4m3x2_to_half2(x), e4m3x2_to_half2(x >> 16), e4m3x2_to_half2(y), e4m3x2_to_half2(y >> 16)};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_f16_16816(o[c][nt], a, pb[nt][0], pb[nt][1]);
-        }
-      }
+      };
+      if (whole) group(std::true_type{}); else group(std::false_type{});
       // ---- the stage is read: the group kPgStages on takes it ----
       __syncwarp();
       const int kf_ = k + kPgStages;
-      if (kf_ < groups) fill(cur, unit0, kf_ / NB == k / NB ? bat : bat_next, kf_);
+      if (kf_ < groups) fill(cur, kf_ / NB == k / NB ? bat : bat_next, kf_);
       if ((k + 1) % NB == 0) {
         bat = bat_next;
-        bat_next.entry = look_up(cur, unit0, k + 1 + NB);
+        bat_next.entry = look_up(cur, k + 1 + NB);
         look_up_scales(cur, bat_next);
       }
     }
 
     // the next piece's first groups come while this one's results meet
     const PagesPiece done = cur;
-    const PagesSeq done_seq = cur_seq;
     have = ok && next_piece(at, cur);
-    cur_seq = seq;
     if (have) {
       open_piece();
     }
@@ -573,9 +513,9 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
       }
       s_m[0][tid] = m; s_l[0][tid] = l;
     }
-    const bool direct = done.u_lo == 0 && done.u_hi == done_seq.units;
+    const bool direct = done.first == 0 && done.last == done.seq.units;
     // a piece that begins before this CTA's share uses the CTA's first slot, one that goes on the second
-    float* part = p.partial + ((long long)blockIdx.x * 2 + (done.u_lo == 0 ? 1 : 0)) * Cfg::kPartial;
+    float* part = p.partial + ((long long)blockIdx.x * 2 + (done.first == 0 ? 1 : 0)) * Cfg::kPartial;
     // the outputs meet a part of d at a time: MMA c holds codes 2 c and 2 c + 1 of each lane
     // group's run of D / 8
     constexpr int kParts = Cfg::kParts, CP = KS / kParts, DP = D / kParts;
@@ -601,9 +541,8 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
         for (int w = 0; w < kPgWarps; ++w) acc += s_o[(w * COLS + col) * DP + dd] * s_w[w][col];
         if (direct) {
           const float l = s_l[0][col];
-          const int row = (done.col0 + col) / hg, h = (done.col0 + col) % hg;
           // a row that sees nothing is zero; l is NaN where a score it sees is
-          p.out[((long long)(done_seq.row0 + row) * p.H + done.gh * hg + h) * D + d] =
+          p.out[((long long)done.b * p.H + done.gh * hg + done.col0 + col) * D + d] =
               __float2bfloat16_rn(l == 0.f ? 0.f : acc / l);
         } else {
           part[col * D + d] = acc;
@@ -611,11 +550,10 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
       }
     }
     if (!direct) {
-      if (tid == 0 && done.u_lo == 0) {
-        const long long seg_end = done.seg_at + done_seq.units + kPgSegCost;
+      if (tid == 0 && done.first == 0) {
         PagesRecord r;
-        r.pieces = (int)((seg_end - 1) / share) - (int)blockIdx.x + 1;
-        r.row0 = done_seq.row0; r.head0 = done.gh * hg; r.col0 = done.col0;
+        r.pieces = (int)((done.end_at - 1) / share) - (int)blockIdx.x + 1;
+        r.row0 = done.b; r.head0 = done.gh * hg; r.col0 = done.col0;
         r.cols = done.cols;
         p.records[blockIdx.x] = r;
       }
@@ -694,8 +632,7 @@ __global__ void __launch_bounds__(kFoldWarps * 32) mha_pages_fold_kernel(const P
       l += s_l[w] * f;
       acc += s_o[w][d] * f;
     }
-    const int row = (r.col0 + c) / p.hg, h = (r.col0 + c) - row * p.hg;
-    p.out[((long long)(r.row0 + row) * p.H + r.head0 + h) * D + d] = __float2bfloat16_rn(l == 0.f ? 0.f : acc / l);
+    p.out[((long long)r.row0 * p.H + r.head0 + r.col0 + c) * D + d] = __float2bfloat16_rn(l == 0.f ? 0.f : acc / l);
   }
 }
 
@@ -726,7 +663,8 @@ static bool pages_map(CUtensorMap* map, const PagesParams& p, int D) {
 }
 
 template <int D, int NT>
-static int launch_pages(const PagesParams& p, cudaStream_t stream) {
+static int launch_pages(PagesParams p, cudaStream_t stream) {
+  p.ctas = kSMs * pg_ctas_per_sm(NT);
   CUtensorMap map;
   if (!pages_map(&map, p, D)) return IRON_ERR_UNSUPPORTED;
   constexpr int smem = PgCfg<D, NT>::kSmem;
@@ -744,7 +682,7 @@ static int launch_pages(const PagesParams& p, cudaStream_t stream) {
   fill_pdl_attr(cfg, attr);
   cfg.gridDim = dim3(p.ctas);
   if (cudaLaunchKernelEx(&cfg, mha_pages_kernel<D, NT>, map, p) != cudaSuccess) return IRON_ERR_LAUNCH;
-  cfg.gridDim = dim3(p.ctas, p.row_start || NT * 8 < p.hg ? NT * 8 : p.hg);
+  cfg.gridDim = dim3(p.ctas, NT * 8 < p.hg ? NT * 8 : p.hg);
   cfg.blockDim = dim3(kFoldWarps * 32);
   cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, mha_pages_fold_kernel<D, NT>, p) == cudaSuccess ? IRON_OK : IRON_ERR_LAUNCH;
@@ -787,7 +725,7 @@ static int pages_args(PagesParams& p, const void* q, const void* pool, const flo
   p.lengths = lengths; p.row_start = row_start; p.out = (__nv_bfloat16*)out; p.records = (PagesRecord*)workspace;
   p.partial = (float*)(p.records + kPgCtas);
   p.B = B; p.H = H; p.G = G; p.hg = H / G; p.P = P; p.width = width; p.log_page = log_page; p.causal = causal; p.window = window;
-  p.rows = rows; p.ctas = kPgCtas;
+  p.rows = rows;
   p.scale_log2 = scale * 1.4426950408889634f;
   return IRON_OK;
 }
