@@ -286,6 +286,8 @@ def test_decode_many_short_and_a_few_long():
     (24, 8, 128, 64, [513, 2, 77], [512, 2, 76]),
     (12, 1, 64, 256, [300, 900], [300, 11]),
     (3, 3, 128, 32, [1000], [1000]),
+    (8, 2, 128, 64, [1000, 129, 2500, 128, 256, 257], [3, 1, 9, 32, 32, 33]),   # one half of an item's columns or fewer
+    (32, 2, 64, 16, [4000, 130, 385], [8, 5, 9]),
 ])
 @pytest.mark.parametrize("mask", ["causal", "window 0", "window 50", "all"])
 def test_prefill(H, G, D, page, lengths, new, mask):
