@@ -638,7 +638,8 @@ int iron_rope_kv_pages_e4m3(const void* qkv, long long pitch, const void* angles
 
 /* One query a request, q (B, H, D), over its cache: out = softmax(scale * q K^T) V, f32 inside.
  * window >= 0 keeps the keys within `window` positions of the last.  A request of length 0 gets
- * zeros.  `workspace` (iron_mha_pages_workspace_bytes(D, 0) bytes, 16-byte aligned) holds the call's
+ * zeros, and so does a query all of whose scores are -infinity.  A length past width * page counts
+ * as that.  `workspace` (iron_mha_pages_workspace_bytes(D, 0) bytes, 16-byte aligned) holds the call's
  * partial results; it needs no clearing, and two calls that may overlap need one each.  `status`
  * (may be NULL) receives IRON_ERR_TIMEOUT when a bounded wait of the pipeline gives up. */
 long long iron_mha_pages_workspace_bytes(int D, int prompt);

@@ -711,8 +711,11 @@ static int pages_args(PagesParams& p, const void* q, const void* pool, const flo
   const int log_page = log2_page(page_size);
   if (B < 0 || rows < 0 || H <= 0 || G <= 0 || H % G || (D != 64 && D != 128) || P <= 0 || width <= 0 || log_page < 0)
     return IRON_ERR_SHAPE;
-  if (G > 65535 || (long long)P * G * (page_size / 8) > 0x7fffffffll || (long long)P * page_size > 0x7fffffffll || (long long)rows * H > 0x7fffffffll) return IRON_ERR_SHAPE;
-  if ((long long)width * page_size > 0x7fffffffll) return IRON_ERR_SHAPE;
+  // indices of 16-token units, tokens and columns are 32-bit, with room for a tile's or an item's end
+  constexpr long long kMost = 0x7fffffffll - 1023;
+  if (G > 65535 || (long long)P * G * (page_size / 8) > kMost || (long long)P * page_size > kMost ||
+      (long long)width * page_size > kMost || (long long)rows * H > kMost)
+    return IRON_ERR_SHAPE;
   if (window >= 0 && !causal) return IRON_ERR_UNSUPPORTED;
   if (!(scale > 0.f)) return IRON_ERR_SHAPE;
   if (B == 0 || rows == 0) return 1;   // nothing to do
@@ -724,7 +727,8 @@ static int pages_args(PagesParams& p, const void* q, const void* pool, const flo
   p.q = (const __nv_bfloat16*)q; p.pool = (const uint8_t*)pool; p.scales = scales; p.tables = tables;
   p.lengths = lengths; p.row_start = row_start; p.out = (__nv_bfloat16*)out; p.records = (PagesRecord*)workspace;
   p.partial = (float*)(p.records + kPgCtas);
-  p.B = B; p.H = H; p.G = G; p.hg = H / G; p.P = P; p.width = width; p.log_page = log_page; p.causal = causal; p.window = window;
+  p.B = B; p.H = H; p.G = G; p.hg = H / G; p.P = P; p.width = width; p.log_page = log_page; p.causal = causal;
+  p.window = window < (long long)width * page_size ? window : -1;   // one that leaves nothing out is none: no difference wraps
   p.rows = rows;
   p.scale_log2 = scale * 1.4426950408889634f;
   return IRON_OK;

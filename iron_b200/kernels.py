@@ -684,6 +684,11 @@ def pages_workspace(D: int, prompt: bool = False, device=None) -> torch.Tensor:
     return torch.empty(n, dtype=torch.uint8, device=device or "cuda")
 
 
+def _window(window) -> int:
+    """A window as the C entries take it: -1 for none, and what passes 32 bits leaves nothing out either."""
+    return -1 if window is None else min(int(window), 2**31 - 1)
+
+
 def _pages_attention(Q, pool, scales, tables, lengths, out, workspace, row_start=None):
     _bf16(Q, out)
     P, G, page, D = _pool_sizes(pool, scales)
@@ -713,7 +718,7 @@ def mha_decode_pages(Q, pool, scales, tables, lengths, out=None, *, window=None,
         raise ValueError(f"Q {tuple(Q.shape)} is not one query for each of {tuple(lengths.shape)} requests")
     P, G, page, D, out, workspace, stream = _pages_attention(Q, pool, scales, tables, lengths, out, workspace)
     call("iron_mha_decode_pages_bf16", Q.data_ptr(), pool.data_ptr(), scales.data_ptr(), P, page, tables.data_ptr(),
-         tables.shape[1], lengths.data_ptr(), Q.shape[0], Q.shape[1], G, D, -1 if window is None else int(window),
+         tables.shape[1], lengths.data_ptr(), Q.shape[0], Q.shape[1], G, D, _window(window),
          1.0 / math.sqrt(D) if scale is None else float(scale), workspace.data_ptr(), workspace.numel(),
          out.data_ptr(), _ptr(status), stream)
     return out
@@ -734,7 +739,7 @@ def mha_prefill_pages(Q, pool, scales, tables, lengths, row_start, out=None, *, 
     P, G, page, D, out, workspace, stream = _pages_attention(Q, pool, scales, tables, lengths, out, workspace, row_start)
     call("iron_mha_prefill_pages_bf16", Q.data_ptr(), pool.data_ptr(), scales.data_ptr(), P, page, tables.data_ptr(),
          tables.shape[1], lengths.data_ptr(), row_start.data_ptr(), B, Q.shape[0], Q.shape[1], G, D, int(bool(causal)),
-         -1 if window is None else int(window), 1.0 / math.sqrt(D) if scale is None else float(scale),
+         _window(window), 1.0 / math.sqrt(D) if scale is None else float(scale),
          workspace.data_ptr(), workspace.numel(), out.data_ptr(), _ptr(status), stream)
     return out
 

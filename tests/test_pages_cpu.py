@@ -121,6 +121,9 @@ def test_the_c_entries_refuse_before_any_launch():
     assert attend(H=5) == attend(D=80) == attend(page=17) == attend(scale=0.0) == attend(scale=float("nan")) == shape
     assert attend(q=None) == attend(starts=None) == attend(rows=-1) == shape
     assert attend(q=8) == align and attend(causal=0, window=3) == unsup and attend(nbytes=100) == small
+    wide = lambda width, P: lib.iron_mha_prefill_pages_bf16(a, a, a, P, 16, a, width, a, a, 2, 2, 4, 2, 64, 1, -1, 1.0,  # noqa: E731
+                                                            a, 1 << 40, a, None, None)
+    assert wide(1 << 27, 4) == wide((1 << 27) - 1, 4) == wide(1, 1 << 27) == shape       # indices past 2^31
     assert attend(B=0, q=None) == attend(rows=0, q=None) == 0
     assert lib.iron_mha_decode_pages_bf16(a, a, a, 4, 16, a, 1, a, 2, 6, 4, 64, -1, 1.0, a, 1 << 40, a, None, None) == shape
     assert lib.iron_mha_pages_workspace_bytes(96, 0) == 0 < lib.iron_mha_pages_workspace_bytes(64, 0) < lib.iron_mha_pages_workspace_bytes(64, 1)

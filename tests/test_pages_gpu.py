@@ -112,6 +112,22 @@ def test_page_step_survives_a_ring_that_says_nonsense():
     assert t.shape == before.shape and torch.cuda.synchronize() is None
 
 
+def test_page_step_of_as_many_requests_as_it_takes():
+    from iron_b200 import _lib
+    from iron_b200 import kernels as K
+
+    B, width, page, rows = _lib.load().iron_page_step_max_requests(), 7, 16, 30000
+    tables, lengths, new, pages, ring = step_inputs(B, width, page, 1, 9000, 0.2, 6)
+    want = R.page_step(tables, lengths, new, pages, ring, page, rows)
+    t, l, n, p, r = map(ints, (tables, lengths, new, pages, ring))
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):                          # a stream other than the one that made the inputs
+        got = K.page_step(t, l, n, p, r, page_size=page, rows=rows, lengths_out=l, ring_out=r)
+    stream.synchronize()
+    check_step(got, t, p, want)
+
+
 # ---------------------------------------------------------------------------- rope_kv_pages
 def write_case(H, G, D, page, before, new, seed, wild=False):
     """Requests with ``before`` tokens bring ``new`` rows; the pool holds the pages the step touches."""
@@ -321,6 +337,61 @@ def test_more_rows_than_keys_and_rows_that_see_nothing(D):
     assert (out[:7] == 0).all() and (out[10:14] == 0).all()
     out = K.mha_prefill_pages(q, pool, scales, t, ints(lengths), ints(start), causal=False)
     check_attention(out, *R.attention(q, pool, scales, t, lengths, start, causal=False))
+
+
+@pytest.mark.parametrize("window", [2**31 - 1, 2**31 - 30, 2**33, 80])
+def test_a_window_wider_than_the_cache_is_none(window):
+    """Rows before the first key and a window near the largest integer: no difference of the two wraps."""
+    from iron_b200 import kernels as K
+
+    lengths, start, page = [3, 40], [0, 50, 120], 16
+    tables, P = R.tables_for(lengths, page, 1)
+    pool, scales = R.cache(P, 2, page, 64, 3)
+    q, t, l = queries(120, 4, 64, 1), ints(tables), ints(lengths)
+    check_attention(K.mha_prefill_pages(q, pool, scales, t, l, ints(start), window=window),
+                    *R.attention(q, pool, scales, t, lengths, start))
+    check_attention(K.mha_decode_pages(q[:2], pool, scales, t, l, window=window),
+                    *R.attention(q[:2], pool, scales, t, lengths, range(3)))
+
+
+@pytest.mark.parametrize("H, G, D", [(8, 2, 64), (10, 2, 128)])
+def test_many_requests_most_of_which_bring_nothing(H, G, D):
+    """Hundreds of requests: more than a CTA has threads, rows of some of them far apart, lengths past the table."""
+    from iron_b200 import kernels as K
+
+    rng = np.random.default_rng(4)
+    B, page, width = 700, 16, 6
+    lengths = np.where(rng.random(B) < 0.3, 0, rng.integers(1, width * page + 1, B))
+    new = np.where(rng.random(B) < 0.9, 0, np.minimum(lengths, rng.integers(0, 90, B)))
+    new[:200] = new[400:600] = 0
+    tables, P = R.tables_for(lengths, page, 1, width=width)
+    pool, scales = R.cache(P, G, page, D, 3)
+    start, t = np.concatenate(([0], np.cumsum(new))), ints(tables)
+    told = ints(np.where(lengths == width * page, lengths + 1000, lengths))
+    q = queries(max(B, int(start[-1])), H, D, 1)
+    n = int(start[-1])
+    out = K.mha_prefill_pages(q[:n], pool, scales, t, told, ints(start))
+    check_attention(out, *R.attention(q[:n], pool, scales, t, lengths, start))
+    out = K.mha_decode_pages(q[:B], pool, scales, t, told)
+    check_attention(out, *R.attention(q[:B], pool, scales, t, lengths, range(B + 1)))
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+def test_queries_that_are_not_finite(prompt):
+    """An infinite or NaN query spoils its own row and head, and no other."""
+    from iron_b200 import kernels as K
+
+    n, page, G, H, D = 200, 16, 2, 8, 64
+    tables, P = R.tables_for([n], page, 1)
+    pool, scales = R.cache(P, G, page, D, 3)
+    m = 150 if prompt else 1
+    q, t, l = queries(m, H, D, 1), ints(tables), ints([n])
+    want, size = R.attention(q, pool, scales, t, [n], [0, m])
+    bad = q.clone()
+    bad[0, 1, 3], bad[m - 1, 6, 0] = float("nan"), float("nan")
+    out = K.mha_prefill_pages(bad, pool, scales, t, l, ints([0, m])) if prompt else K.mha_decode_pages(bad, pool, scales, t, l)
+    want[0, 1], want[m - 1, 6] = float("nan"), float("nan")
+    check_attention(out, want, size)
 
 
 @pytest.mark.parametrize("D", [64, 128])
