@@ -109,7 +109,7 @@ __device__ __forceinline__ long long warp_sum_ll(long long v) {
   return v;
 }
 
-// The items of [at, end) of the dealt-out cost, in order.
+// The items of [at, end) of the dealt-out cost, in order, as one warp walks them.
 struct PtWalk {
   int b, g, j;
   long long at, end;       // where item (b, g, j) begins; the share's end
@@ -117,11 +117,18 @@ struct PtWalk {
   PtSeq seq;
   __device__ __forceinline__ bool next(const PagesParams& p, PtItem& x) {
     while (at < end) {
-      while (j >= seq.blocks) {
+      if (j >= seq.blocks) {
         j = 0;
-        if (seq.blocks == 0 || ++g >= p.G) {
+        if (++g >= p.G) {
           g = 0;
           seq = pt_seq(p, ++b);
+          while (seq.blocks == 0) {
+            // the next sequence with rows, 32 at a look
+            const int lane = threadIdx.x & 31;
+            const unsigned some = __ballot_sync(0xffffffffu, b + lane < p.B && pt_seq(p, b + lane).blocks > 0);
+            if (some) seq = pt_seq(p, b += __ffs(some) - 1);
+            else if ((b += 32) >= p.B) return false;
+          }
         }
       }
       pt_block(p, seq, j, x);
@@ -278,18 +285,43 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
 
   pdl_launch();
   pdl_wait();
-  // ---- where this CTA's share begins: a warp sums a stretch of the sequences, a lane their blocks ----
+  // ---- where this CTA's share begins: a warp sums a stretch of the sequences, 32 at a look ----
   const int per_warp = (p.B + kWarps - 1) / kWarps;
   const int sb = min(warp * per_warp, p.B), se = min(sb + per_warp, p.B);
-  long long mine = 0;
-  for (int b = sb; b < se; ++b) {
-    const PtSeq s = pt_seq(p, b);
-    for (int j = lane; j < s.blocks; j += 32) {
-      PtItem x;
-      pt_block(p, s, j, x);
-      mine += pt_cost(x);
+  auto seq_at = [&](int b) {
+    PtSeq s = {};
+    if (b < se) s = pt_seq(p, b);
+    return s;
+  };
+  // every lane its sequence's cost of one KV head: one block is the lane's own to count, more are the warp's
+  auto costs = [&](const PtSeq& s) {
+    PtItem x;
+    long long own = 0;
+    if (s.blocks == 1) { pt_block(p, s, 0, x); own = pt_cost(x); }
+    for (unsigned left = __ballot_sync(0xffffffffu, s.blocks > 1); left; left &= left - 1) {
+      const int l = __ffs(left) - 1;
+      PtSeq y = {};
+      y.len = __shfl_sync(0xffffffffu, s.len, l);
+      y.n = __shfl_sync(0xffffffffu, s.n, l);
+      y.blocks = __shfl_sync(0xffffffffu, s.blocks, l);
+      long long c = 0;
+      for (int j = lane; j < y.blocks; j += 32) { pt_block(p, y, j, x); c += pt_cost(x); }
+      c = warp_sum_ll(c);
+      if (lane == l) own = c;
     }
-  }
+    return own;
+  };
+  // sums over the lanes up to and with one's own
+  auto upto_lane = [&](long long v) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += y;
+    }
+    return v;
+  };
+  long long mine = 0;
+  for (int b0 = sb; b0 < se; b0 += 32) mine += costs(seq_at(b0 + lane));
   mine = warp_sum_ll(mine) * p.G;
   if (lane == 0) s_sum[warp] = mine;
   if (tid == 0) { s_nan = 0; p.records[blockIdx.x].pieces = 0; }
@@ -304,34 +336,28 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
   if (begin >= end) return;
   if (begin >= before && begin < before + mine) {
     long long acc = before;
-    for (int b = sb; b < se; ++b) {
-      const PtSeq s = pt_seq(p, b);
-      long long one = 0;
-      for (int j = lane; j < s.blocks; j += 32) {
-        PtItem x;
-        pt_block(p, s, j, x);
-        one += pt_cost(x);
-      }
-      one = warp_sum_ll(one);
-      if (begin >= acc + one * p.G) { acc += one * p.G; continue; }
+    for (int b0 = sb; b0 < se; b0 += 32) {
+      PtSeq s = seq_at(b0 + lane);
+      const long long own = costs(s), upto = upto_lane(own * p.G);
+      const unsigned hit = __ballot_sync(0xffffffffu, begin < acc + upto);
+      if (!hit) { acc += __shfl_sync(0xffffffffu, upto, 31); continue; }
+      const int l = __ffs(hit) - 1;
+      const long long one = __shfl_sync(0xffffffffu, own, l);
+      acc += __shfl_sync(0xffffffffu, upto, l) - one * p.G;
       const int g = (int)((begin - acc) / one);
       acc += one * g;
+      s = pt_seq(p, b0 + l);
       for (int j0 = 0; j0 < s.blocks; j0 += 32) {
         PtItem x;
         int cost = 0;
         if (j0 + lane < s.blocks) { pt_block(p, s, j0 + lane, x); cost = pt_cost(x); }
-        long long upto = cost;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const long long y = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += y;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, cost > 0 && begin < acc + upto);
-        if (hit) {
-          if (lane == __ffs(hit) - 1) { s_b = b; s_g = g; s_j = j0 + lane; s_at = acc + upto - cost; }
+        const long long so_far = upto_lane(cost);
+        const unsigned in = __ballot_sync(0xffffffffu, cost > 0 && begin < acc + so_far);
+        if (in) {
+          if (lane == __ffs(in) - 1) { s_b = b0 + l; s_g = g; s_j = j0 + lane; s_at = acc + so_far - cost; }
           break;
         }
-        acc += __shfl_sync(0xffffffffu, upto, 31);
+        acc += __shfl_sync(0xffffffffu, so_far, 31);
       }
       break;
     }
@@ -507,23 +533,27 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
     uint64_t* full = values ? v_full : k_full;
     uint64_t* empty = values ? v_empty : k_empty;
     uint8_t* tiles = smem + (values ? Cfg::kV : Cfg::kK);
-    struct Tile { int key0, any_lo, any_hi, gh, entry; bool partial; };
+    // What is kept of a tile beside its codes, in few registers: the rows that some column sees
+    // [lo, hi), whether some column does not see all of them, and where this lane's 16 keys begin in their
+    // page (in sixteens).
+    auto tile_word = [](int lo, int hi, bool partial, int off) { return lo | hi << 8 | (partial ? 1 << 16 : 0) | off << 17; };
     PtItem it;
     int t_at = 0;
     bool have_item = false;
     auto take = [&](const PtItem& x) { it = x; };
-    auto advance = [&](Tile& x) {  // the next tile of the share; false at its end
+    int entry = -1, word = 0;      // of the next tile: this lane's page id, then its unit in the pool
+    auto advance = [&]() {         // the next tile of the share; false at its end
       while (!have_item || t_at >= it.t_hi) {
         if (!next_item(take)) return false;
         have_item = true;
         t_at = it.t_lo;
       }
-      x.key0 = (it.tile0 + t_at) * kPtKeys;
-      x.any_lo = it.any_lo; x.any_hi = it.any_hi; x.gh = it.gh;
-      x.partial = x.key0 < it.all_lo || x.key0 + kPtKeys > it.all_hi;
-      const int key = x.key0 + 32 * w + 16 * (lane & 1);      // even lanes: the warp's first 16 keys
-      x.entry = -1;
-      if (key < it.any_hi) x.entry = p.tables[(long long)it.b * p.width + (key >> p.log_page)];
+      const int key0 = (it.tile0 + t_at) * kPtKeys;
+      const int key = key0 + 32 * w + 16 * (lane & 1);      // even lanes: the warp's first 16 keys
+      entry = -1;
+      if (key < it.any_hi) entry = p.tables[(long long)it.b * p.width + (key >> p.log_page)];
+      word = tile_word(max(it.any_lo - key0, 0), min(max(it.any_hi - key0, 0), kPtKeys),
+                       key0 < it.all_lo || key0 + kPtKeys > it.all_hi, (key & ((1 << p.log_page) - 1)) >> 4);
       ++t_at;
       return true;
     };
@@ -532,10 +562,10 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
     const int at0 = (piece >> 2) * kPtSub + (32 * w + sub_row) * 128, chunk = 2 * (piece & 3);
     const uint8_t* my_codes = p.pool + sub_row * D + piece * 16;
     // A tile's page ids come as the index of a 16-token unit of one page, KV head and kind.
-    auto load = [&](const Tile& x) {
+    auto load = [&]() {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int unit = __shfl_sync(0xffffffffu, x.entry, half);
+        const int unit = __shfl_sync(0xffffffffu, entry, half);
         const uint8_t* base = my_codes + (long long)max(unit, 0) * (16 * D);
 #pragma unroll
         for (int k = 0; k < kReps / 2; ++k)
@@ -543,14 +573,13 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
       }
     };
     float2 scale = make_float2(1.f, 0.f);
-    auto unit_of = [&](Tile& x) {
-      const int off = (x.key0 + 32 * w + 16 * (lane & 1)) & ((1 << p.log_page) - 1);
-      const bool there = x.entry >= 0 && x.entry < p.P;
+    auto unit_of = [&]() {
+      const bool there = entry >= 0 && entry < p.P;
       // an absent page: its scores are -inf through the logarithm, its share of the sum nothing
       scale = make_float2(1.f, 0.f);
       if (!values && there && lane < 2)
-        scale = *reinterpret_cast<const float2*>(p.scales + ((long long)x.entry * p.G + x.gh) * 2);
-      x.entry = there ? (((x.entry * p.G + x.gh) * 2 + (values ? 1 : 0)) << (p.log_page - 4)) + (off >> 4) : -1;
+        scale = *reinterpret_cast<const float2*>(p.scales + ((long long)entry * p.G + it.gh) * 2);
+      entry = there ? (((entry * p.G + it.gh) * 2 + (values ? 1 : 0)) << (p.log_page - 4)) + (word >> 17) : -1;
     };
     auto store = [&](uint8_t* tile, int k, const uint4& c) {
       const int row7 = (k * kRowsAtOnce + sub_row) & 7;
@@ -560,12 +589,13 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
       *reinterpret_cast<uint4*>(dst + ((chunk ^ row7) << 4)) = lo;
       *reinterpret_cast<uint4*>(dst + (((chunk + 1) ^ row7) << 4)) = hi;
     };
-    Tile now, nxt;
-    bool have = advance(now), more = false;
+    int now = 0;                // the word of the tile whose codes are held
+    bool have = advance(), more = false;
     if (have) {
-      unit_of(now);
-      load(now);
-      more = advance(nxt);      // its page ids are there by the time its loads begin
+      unit_of();
+      load();
+      now = word;
+      more = advance();         // its page ids are there by the time its loads begin
     }
     int s = 0, n_tile = 0;
     uint32_t ph = 0;
@@ -573,14 +603,14 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
       ok = mbar_wait_relaxed(empty + s, ph ^ 1, abort_flag, 64);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      if (values && now.partial) {
+      if (values && (now >> 16 & 1)) {
         // values that no column sees count as zero; a NaN that some see is zero here and comes
         // back where it is seen when the outputs are written
 #pragma unroll
         for (int k = 0; k < kReps; ++k) {
-          const int key = now.key0 + 32 * w + k * kRowsAtOnce + sub_row;
+          const int row = 32 * w + k * kRowsAtOnce + sub_row;
           uint32_t* c = reinterpret_cast<uint32_t*>(&codes[k]);
-          if (key < now.any_lo || key >= now.any_hi) codes[k] = make_uint4(0, 0, 0, 0);
+          if (row < (now & 0xff) || row >= (now >> 8 & 0xff)) codes[k] = make_uint4(0, 0, 0, 0);
           if (nan_codes(c[0]) | nan_codes(c[1]) | nan_codes(c[2]) | nan_codes(c[3])) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) c[q] &= ~((nan_codes(c[q]) >> 7) * 0xffu);
@@ -603,13 +633,13 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(full + s);
       if (more) {
-        unit_of(nxt);
-        load(nxt);
+        unit_of();
+        load();
       }
       if (++s == Cfg::kStages) { s = 0; ph ^= 1; }
-      now = nxt;
+      now = word;
       have = more;
-      if (more) more = advance(nxt);
+      if (more) more = advance();
     }
   } else {
     // ---------------- softmax and output ----------------
