@@ -51,14 +51,16 @@ constexpr float kPgLift = 10.f;             // log2 of what probabilities are he
 // many units a segment -- a KV head's group of columns -- has.  An empty one still has a unit:
 // somebody must write its zeros.
 struct PagesSeq {
-  int len, lo, unit0, units;
+  int len, lo, unit0, units, row;   // row: of q and of the outputs
 };
 __device__ __forceinline__ PagesSeq pages_seq(const PagesParams& p, int b) {
   PagesSeq s;
-  s.len = max(0, (int)min((long long)p.lengths[b], (long long)p.width << p.log_page));
+  s.len = seq_len(p, b);
+  s.row = b;
   s.lo = p.window >= 0 ? max(0, s.len - 1 - p.window) : 0;
   s.unit0 = s.lo / kPgUnit;
   s.units = max(1, (s.len + kPgUnit - 1) / kPgUnit - s.unit0);
+  if (p.row_start && seq_rows(p, b, s.row) != 1) s.units = 0;   // ragged rows: those of one row are this kernel's
   return s;
 }
 
@@ -78,7 +80,7 @@ struct PgCfg {
 
 // what a sequence's segments cost in units; `segs`: KV heads times groups of columns
 __device__ __forceinline__ long long pages_cost(int segs, const PagesSeq& s) {
-  return (long long)segs * (s.units + kPgSegCost);
+  return s.units ? (long long)segs * (s.units + kPgSegCost) : 0;
 }
 
 // units per CTA: an equal share, and two groups a warp at least
@@ -206,6 +208,11 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
       for (long long w; at >= seq_at + (w = pages_cost(segs, seq));) {
         seq_at += w;
         seq = pages_seq(p, ++seq_b);
+        while (seq.units == 0) {      // the next that has some, 32 at a look
+          const unsigned some = __ballot_sync(0xffffffffu, seq_b + lane < p.B && pages_seq(p, seq_b + lane).units > 0);
+          if (some) seq = pages_seq(p, seq_b += __ffs(some) - 1);
+          else if ((seq_b += 32) >= p.B) return false;
+        }
       }
       const int span = seq.units + kPgSegCost;
       const int seg = (int)div_ll(at - seq_at, span);
@@ -276,7 +283,7 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int c = nt * 8 + g;
-      const __nv_bfloat16* src = p.q + ((long long)cur.b * p.H + cur.gh * hg + cur.col0 + c) * D + t * (D / 4);
+      const __nv_bfloat16* src = p.q + ((long long)cur.seq.row * p.H + cur.gh * hg + cur.col0 + c) * D + t * (D / 4);
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) q_raw[nt][i] = c < cur.cols ? ld_cached(src + 8 * i) : make_uint4(0, 0, 0, 0);
     }
@@ -542,7 +549,7 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
         if (direct) {
           const float l = s_l[0][col];
           // a row that sees nothing is zero; l is NaN where a score it sees is
-          p.out[((long long)done.b * p.H + done.gh * hg + done.col0 + col) * D + d] =
+          p.out[((long long)done.seq.row * p.H + done.gh * hg + done.col0 + col) * D + d] =
               __float2bfloat16_rn(l == 0.f ? 0.f : acc / l);
         } else {
           part[col * D + d] = acc;
@@ -553,7 +560,7 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
       if (tid == 0 && done.first == 0) {
         PagesRecord r;
         r.pieces = (int)((done.end_at - 1) / share) - (int)blockIdx.x + 1;
-        r.row0 = done.b; r.head0 = done.gh * hg; r.col0 = done.col0;
+        r.row0 = done.seq.row; r.head0 = done.gh * hg; r.col0 = done.col0;
         r.cols = done.cols;
         p.records[blockIdx.x] = r;
       }
@@ -693,15 +700,19 @@ static int launch_pages_cols(const PagesParams& p, int cols, cudaStream_t stream
   return cols <= 8 ? launch_pages<D, 1>(p, stream) : launch_pages<D, 2>(p, stream);
 }
 
+static int launch_decode(const PagesParams& p, int D, cudaStream_t stream) {
+  return D == 64 ? launch_pages_cols<64>(p, p.hg, stream) : launch_pages_cols<128>(p, p.hg, stream);
+}
+
 }  // namespace iron
 
 using namespace iron;
 
 extern "C" long long iron_mha_pages_workspace_bytes(int D, int prompt) {
   if (D != 64 && D != 128) return 0;
-  if (prompt) return mha_pages_tc_workspace_bytes(D);
   const long long partial = 16ll * D + 32;
-  return (long long)kPgCtas * (2 * partial * (long long)sizeof(float) + (long long)sizeof(PagesRecord));
+  return (prompt ? mha_pages_tc_workspace_bytes(D) : 0) +
+         (long long)kPgCtas * (2 * partial * (long long)sizeof(float) + (long long)sizeof(PagesRecord));
 }
 
 static int pages_args(PagesParams& p, const void* q, const void* pool, const float* scales, int P, int page_size,
@@ -725,7 +736,8 @@ static int pages_args(PagesParams& p, const void* q, const void* pool, const flo
     return IRON_ERR_ALIGN;
   if (workspace_bytes < iron_mha_pages_workspace_bytes(D, row_start != nullptr)) return IRON_ERR_WORKSPACE;
   p.q = (const __nv_bfloat16*)q; p.pool = (const uint8_t*)pool; p.scales = scales; p.tables = tables;
-  p.lengths = lengths; p.row_start = row_start; p.out = (__nv_bfloat16*)out; p.records = (PagesRecord*)workspace;
+  p.lengths = lengths; p.row_start = row_start; p.out = (__nv_bfloat16*)out;
+  p.records = (PagesRecord*)((char*)workspace + (row_start ? mha_pages_tc_workspace_bytes(D) : 0));
   p.partial = (float*)(p.records + kPgCtas);
   p.B = B; p.H = H; p.G = G; p.hg = H / G; p.P = P; p.width = width; p.log_page = log_page; p.causal = causal;
   p.window = window < (long long)width * page_size ? window : -1;   // one that leaves nothing out is none: no difference wraps
@@ -743,7 +755,7 @@ extern "C" int iron_mha_decode_pages_bf16(const void* q, const void* pool, const
                             scale, workspace, workspace_bytes, out);
   if (rc) return rc == 1 ? IRON_OK : rc;
   p.status = status;
-  return D == 64 ? launch_pages_cols<64>(p, H / G, (cudaStream_t)stream) : launch_pages_cols<128>(p, H / G, (cudaStream_t)stream);
+  return launch_decode(p, D, (cudaStream_t)stream);
 }
 
 extern "C" int iron_mha_prefill_pages_bf16(const void* q, const void* pool, const float* scales, int P, int page_size,
@@ -756,5 +768,14 @@ extern "C" int iron_mha_prefill_pages_bf16(const void* q, const void* pool, cons
   if (rc) return rc == 1 ? IRON_OK : rc;
   if (!row_start) return IRON_ERR_SHAPE;
   p.status = status;
-  return mha_pages_tc(p, D, workspace, (cudaStream_t)stream);
+  // A sequence of one row fills hg of the ragged kernel's 128 lanes, the decode kernel's eight columns
+  // well.  32 heads over 8 of 128, pages of 64, without and with the split: 256 x 1 row on 300 tokens
+  // 187 and 67 us, 64 x 1 on 3000 185 and 80, 16 x 1 on 300 27.6 and 21.5; where no sequence has one row
+  // the decode kernel's launches are lost (8 x 64 rows on 1000: 43.0 and 49.2 us; 64 x 33: 118 and 123).
+  // How many there are is known on the device alone, so: where there may be many, and where there
+  // can be nothing else.
+  p.split = B > 16 || rows == 1;
+  if (rows > 1)
+    if (const int bad = mha_pages_tc(p, D, workspace, (cudaStream_t)stream)) return bad;
+  return p.split ? launch_decode(p, D, (cudaStream_t)stream) : IRON_OK;
 }

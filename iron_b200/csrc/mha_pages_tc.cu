@@ -41,7 +41,7 @@ constexpr int kPtSub = 16384;         // a 128-row x 128-byte swizzled sub-tile
 // What the tiles of one and of two 128-column halves cost, and an item beside its tiles, as measured:
 // one half alone waits for its own chain of products and exponentials.
 constexpr int kPtCostOne = 3, kPtCostTwo = 4, kPtItemCost = 12;
-constexpr int kPtMinShare = 36;
+constexpr int kPtMinShare = 12;
 constexpr float kPtLift = 6.f;        // log2 of what weights are held times
 constexpr float kPtSlack = 8.f;       // log2 of how far the maximum in use may lag
 constexpr int kPtFoldWarps = 8;
@@ -73,9 +73,9 @@ struct PtSeq {
 };
 __device__ __forceinline__ PtSeq pt_seq(const PagesParams& p, int b) {
   PtSeq s;
-  s.len = max(0, (int)min((long long)p.lengths[b], (long long)p.width << p.log_page));
-  s.row0 = min(max(p.row_start[b], 0), p.rows);
-  s.n = max(0, min(p.row_start[b + 1], p.rows) - s.row0);
+  s.len = seq_len(p, b);
+  s.n = seq_rows(p, b, s.row0);
+  if (p.split && s.n == 1) s.n = 0;    // the decode kernel's
   s.blocks = (s.n * p.hg + kPtRows - 1) / kPtRows;
   return s;
 }

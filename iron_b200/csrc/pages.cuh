@@ -57,14 +57,24 @@ struct PagesParams {
   const float* scales;
   const int* tables;
   const int* lengths;
-  const int* row_start;     // nullptr: one query a sequence
+  const int* row_start;     // nullptr: one query a sequence, in order
   __nv_bfloat16* out;
   float* partial;
   PagesRecord* records;
   int B, H, G, hg, P, width, log_page, causal, window, rows, ctas;   // hg = H / G
+  int split;                // sequences of one row are the decode kernel's, not the ragged one's
   float scale_log2;
   int* status;
 };
+
+// A sequence's tokens as far as its table goes, and the query rows it brings, inside the buffer.
+__device__ __forceinline__ int seq_len(const PagesParams& p, int b) {
+  return max(0, (int)min((long long)p.lengths[b], (long long)p.width << p.log_page));
+}
+__device__ __forceinline__ int seq_rows(const PagesParams& p, int b, int& row0) {
+  row0 = min(max(p.row_start[b], 0), p.rows);
+  return max(0, min(p.row_start[b + 1], p.rows) - row0);
+}
 
 // a / b for a >= 0, b > 0: the 64-bit division is a long routine, and seldom needed
 __device__ __forceinline__ long long div_ll(long long a, int b) {

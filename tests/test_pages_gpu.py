@@ -376,6 +376,30 @@ def test_many_requests_most_of_which_bring_nothing(H, G, D):
     check_attention(out, *R.attention(q[:B], pool, scales, t, lengths, range(B + 1)))
 
 
+@pytest.mark.parametrize("H, G, D, page", [(8, 2, 64, 16), (32, 2, 128, 64), (5, 5, 128, 32)])
+@pytest.mark.parametrize("lengths, new", [
+    ([700], [1]), ([0], [1]), ([5, 300, 1], [1, 1, 1]), ([0, 40, 1000, 17, 2000, 64], [1, 1, 300, 1, 0, 2]),
+    ([100 + 7 * i for i in range(70)], [1 if i % 3 else 0 for i in range(70)]),
+    ([3000] + [0] * 100 + [64, 4097], [1] + [0] * 100 + [64, 1])])
+@pytest.mark.parametrize("kw", [dict(), dict(window=33), dict(causal=False)], ids=str)
+def test_single_rows_among_others(H, G, D, page, lengths, new, kw):
+    """A step of prompts' rows and of requests that bring one row each."""
+    from iron_b200 import kernels as K
+
+    tables, P = R.tables_for(lengths, page, 5)
+    pool, scales = R.cache(P, G, page, D, 6)
+    poison(pool, scales, tables, lengths, page)
+    start = np.concatenate(([0], np.cumsum(new)))
+    n = int(start[-1])
+    for spare in (0, 2):
+        q = queries(n + spare, H, D, 5)
+        out = torch.full_like(q, 9.0)
+        K.mha_prefill_pages(q, pool, scales, ints(tables), ints(lengths), ints(start), out, **kw)
+        want, size = R.attention(q, pool, scales, ints(tables), lengths, start, **kw)
+        check_attention(out[:n], want[:n], size[:n])
+        assert (out[n:] == 9).all()
+
+
 @pytest.mark.parametrize("prompt", [False, True])
 def test_queries_that_are_not_finite(prompt):
     """An infinite or NaN query spoils its own row and head, and no other."""
