@@ -9,11 +9,12 @@
 //   warps 16, 17  issue S = Q K^T and O += P V for the first and the second 128 columns, each on
 //                 its own so that neither waits for the other's softmax
 //   warps 0..3,   softmax of the first and the second 128 columns: a thread owns a column (one
-//         4..7    lane of tensor memory); scores are read twice, once for the maximum and once for the
-//                 exponentials, and P takes the scores' place in tensor memory as the second
-//                 product's A operand
-// O stays in tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8
-// over the one in use, which after the first tiles is seldom.
+//         4..7    lane of tensor memory) and has a step's 64 scores in registers at once; P takes
+//                 half of their place in tensor memory as the second product's A operand
+//   warp 18       walks the share's items and hands them to all through a ring
+// A tile goes in two steps of 64 keys with a buffer of scores each, so that a step's exponentials are
+// taken while the next one's scores are computed.  O stays in tensor memory; it is rescaled only when
+// a row's maximum has grown by more than 2^8 over the one in use, which after the first tiles is seldom.
 //
 // What the arithmetic is (scales, halves, weights) is the decode kernel's: Q as halves under a
 // power of two a row, a page's key scale on its scores, the logarithm of its value scale added
@@ -25,6 +26,14 @@
 // one a CTA; an item that a boundary cuts leaves partials in the workspace, and a second small
 // launch folds them in order.  Exponentials (16 a clock and SM) and MMAs both need 1024 clocks for
 // 128 columns x 128 keys at D 128.
+//
+// Measured (32 heads over 8): 2048 causal rows, heads of 64: 61 us (282 TFLOP/s); eight chunks of 61 to
+// 1433 rows on 900 to 9001 tokens, heads of 128: 311 us (800 TFLOP/s); 16 x 7 rows on 4096: 74 us.  What
+// bounds the wide items is the softmax's chain: a step takes 2600 clocks of a half (290 until its scores are
+// there, 560 for the maximum, 1250 for the weights, the rest handing over) where exponentials alone would
+// take 1024, the exponentials' pipe is 41 % busy and the tensor pipe 41 %; registers allow no third
+// group of warps to fill it.  Narrow items (few columns) wait for the converters, 5000 clocks a tile; a
+// call has some 14,000 clocks before its first tile and 4000 after an item's last.
 //
 // Every mbarrier wait is bounded; a wait that gives up sets the abort flag, every role unwinds,
 // tensor memory is freed and the status word receives IRON_ERR_TIMEOUT.
@@ -38,9 +47,11 @@ constexpr int kPtThreads = 640;
 constexpr int kPtRows = 256;          // query columns of an item: two 128-row products
 constexpr int kPtKeys = 128;          // keys of a tile
 constexpr int kPtSub = 16384;         // a 128-row x 128-byte swizzled sub-tile
-// What the tiles of one and of two 128-column halves cost, and an item beside its tiles, as measured:
-// one half alone waits for its own chain of products and exponentials.
+// What the tiles of one and of two 128-column halves cost, and an item beside its tiles: one half alone
+// waits for its own chain of products and exponentials.  The eight ragged chunks with 2, 3, 4 for one half:
+// 330, 311, 317 us; with 6, 12, 24 for an item: 345, 311, 317.
 constexpr int kPtCostOne = 3, kPtCostTwo = 4, kPtItemCost = 12;
+// A CTA's share is an item's own cost at least: 8 x 64 rows on 1000 tokens 43 us, with 36 51, with 72 73.
 constexpr int kPtMinShare = 12;
 constexpr float kPtLift = 6.f;        // log2 of what weights are held times
 constexpr float kPtSlack = 8.f;       // log2 of how far the maximum in use may lag
