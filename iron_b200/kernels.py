@@ -597,11 +597,13 @@ def _int32(names: str, *ts) -> None:
 
 def _pool_sizes(pool, scales):
     """(P, G, page, D) of a cache: ``pool`` (P, G, 2, page, D) e4m3, ``scales`` (P, G, 2) float32."""
-    if pool.dtype != E4M3 or scales.dtype != torch.float32:
+    if pool.dtype is not E4M3 or scales.dtype is not torch.float32:
         raise TypeError(f"the pool is float8_e4m3fn and its scales float32, not {pool.dtype} and {scales.dtype}")
-    if pool.dim() != 5 or pool.shape[2] != 2 or scales.shape != pool.shape[:3]:
-        raise ValueError(f"pool {tuple(pool.shape)} and scales {tuple(scales.shape)} are not (P, G, 2, page, D) and (P, G, 2)")
-    return pool.shape[0], pool.shape[1], pool.shape[3], pool.shape[4]
+    shape = pool.shape
+    if len(shape) != 5 or shape[2] != 2 or scales.shape != shape[:3]:
+        raise ValueError(f"pool {tuple(shape)} and scales {tuple(scales.shape)} are not (P, G, 2, page, D) and (P, G, 2)")
+    P, G, _, page, D = shape
+    return P, G, page, D
 
 
 def page_step(tables, lengths, new_tokens, pages, ring, *, page_size, rows, lengths_out=None, ring_out=None,
@@ -624,7 +626,9 @@ def page_step(tables, lengths, new_tokens, pages, ring, *, page_size, rows, leng
     B, width = tables.shape
     if rows < 0:
         raise ValueError(f"rows ({rows}) is negative")
-    if slots is None or positions is None or row_start is None or lengths_out is None or ring_out is None:
+    checked = [tables, lengths, new_tokens, pages, ring]
+    given = [t for t in (slots, positions, row_start, lengths_out, ring_out) if t is not None]
+    if len(given) < 5:
         # one allocation for all that are missing
         made = torch.empty(2 * (B + rows) + 5, dtype=torch.int32, device=tables.device)
         made = torch.split_with_sizes(made, (rows, rows, B + 1, B, 4))
@@ -633,12 +637,14 @@ def page_step(tables, lengths, new_tokens, pages, ring, *, page_size, rows, leng
         row_start = made[2] if row_start is None else row_start
         lengths_out = made[3] if lengths_out is None else lengths_out
         ring_out = made[4] if ring_out is None else ring_out
-    if not (slots.dim() == positions.dim() == row_start.dim() == lengths_out.dim() == ring_out.dim() == 1
-            and slots.numel() == positions.numel() == rows and row_start.numel() == B + 1
-            and lengths_out.numel() == B and ring_out.numel() == 4):
-        raise ValueError("outputs are slots (rows,), positions (rows,), row_start (B + 1,), lengths_out (B,), ring_out (4,)")
-    _int32("page_step's tensors", tables, lengths, new_tokens, pages, ring, slots, positions, row_start, lengths_out, ring_out)
-    stream = _on_device(tables, lengths, new_tokens, pages, ring, slots, positions, row_start, lengths_out, ring_out)
+    if given:
+        if not (slots.dim() == positions.dim() == row_start.dim() == lengths_out.dim() == ring_out.dim() == 1
+                and slots.numel() == positions.numel() == rows and row_start.numel() == B + 1
+                and lengths_out.numel() == B and ring_out.numel() == 4):
+            raise ValueError("outputs are slots (rows,), positions (rows,), row_start (B + 1,), lengths_out (B,), ring_out (4,)")
+        checked += given
+    _int32("page_step's tensors", *checked)
+    stream = _on_device(*checked)
     call("iron_page_step", tables.data_ptr(), width, lengths.data_ptr(), new_tokens.data_ptr(), B, pages.data_ptr(),
          pages.numel(), ring.data_ptr(), page_size, rows, lengths_out.data_ptr(), ring_out.data_ptr(),
          slots.data_ptr(), positions.data_ptr(), row_start.data_ptr(), stream)
@@ -692,19 +698,27 @@ def _window(window) -> int:
 def _pages_attention(Q, pool, scales, tables, lengths, out, workspace, row_start=None):
     _bf16(Q, out)
     P, G, page, D = _pool_sizes(pool, scales)
-    if Q.dim() != 3 or Q.shape[2] != D or Q.shape[1] % G:
-        raise ValueError(f"Q {tuple(Q.shape)} is not (rows, a multiple of {G} heads, {D})")
+    shape = Q.shape
+    if len(shape) != 3 or shape[2] != D or shape[1] % G:
+        raise ValueError(f"Q {tuple(shape)} is not (rows, a multiple of {G} heads, {D})")
     if tables.dim() != 2 or lengths.shape != tables.shape[:1]:
         raise ValueError(f"tables {tuple(tables.shape)} and lengths {tuple(lengths.shape)} are not (B, width) and (B,)")
+    checked = [Q, pool, scales, tables, lengths]
+    if row_start is not None:
+        checked.append(row_start)
+    _int32("tables, lengths and row_start", *checked[3:])
     if out is None:
         out = torch.empty_like(Q)
-    elif out.shape != Q.shape:
-        raise ValueError(f"out {tuple(out.shape)} is not {tuple(Q.shape)}")
+    elif out.shape != shape:
+        raise ValueError(f"out {tuple(out.shape)} is not {tuple(shape)}")
+    else:
+        checked.append(out)
+    if workspace is not None:
+        checked.append(workspace)
+    stream = _on_device(*checked)
     if workspace is None:
         workspace = pages_workspace(D, row_start is not None, Q.device)
-    starts = () if row_start is None else (row_start,)
-    _int32("tables, lengths and row_start", tables, lengths, *starts)
-    return P, G, page, D, out, workspace, _on_device(Q, out, pool, scales, tables, lengths, workspace, *starts)
+    return P, G, page, D, out, workspace, stream
 
 
 def mha_decode_pages(Q, pool, scales, tables, lengths, out=None, *, window=None, scale=None, workspace=None,
