@@ -149,9 +149,7 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
   constexpr int NB = 32 / U;                    // groups whose pages a warp's lanes look up at once
   extern __shared__ uint8_t pg_smem_raw[];
   __shared__ float s_m[kPgWarps][COLS], s_l[kPgWarps][COLS], s_w[kPgWarps][COLS];
-  __shared__ long long s_scan[kPgWarps];
-  __shared__ int s_b, s_abort;
-  __shared__ long long s_at;
+  __shared__ int s_abort;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pg_smem_raw) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int hg = p.hg, page_mask = (1 << p.log_page) - 1;
@@ -168,47 +166,41 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
   }
 
+  __syncthreads();      // the abort flag is there
+  volatile int* abort_flag = &s_abort;
+
   pdl_launch();
   pdl_wait();
-  // where this CTA's run of units begins: every thread sums a stretch of the sequences
-  const int per_thread = (p.B + kPgThreads - 1) / kPgThreads;
-  const int sb = min(tid * per_thread, p.B), se = min(sb + per_thread, p.B);
-  long long mine = 0;
-  for (int b = sb; b < se; ++b) {
-    const PagesSeq s = pages_seq(p, b);
-    mine += pages_cost(segs, s);
-  }
-  long long before = mine, total = 0;
+  // Where this CTA's run of units begins: every warp looks at all sequences for itself, 32 at once, so
+  // that none waits for another.
+  auto seq_cost = [&](int b) { return b < p.B ? pages_cost(segs, pages_seq(p, b)) : 0ll; };
+  long long total = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 32) total += seq_cost(b0 + lane);
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long x = __shfl_up_sync(0xffffffffu, before, o);
-    if (lane >= o) before += x;
-  }
-  if (lane == 31) s_scan[warp] = before;
-  __syncthreads();
-  before -= mine;
-#pragma unroll
-  for (int w = 0; w < kPgWarps; ++w) {
-    if (w < warp) before += s_scan[w];
-    total += s_scan[w];
-  }
+  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   const long long share = pages_share(total, p.ctas);
   const long long begin = (long long)blockIdx.x * share, end = min(begin + share, total);
   if (tid == 0) p.records[blockIdx.x].pieces = 0;   // until this CTA begins a segment that others go on with
   if (begin >= end) return;
-  if (begin >= before && begin < before + mine) {
-    long long acc = before;
-    for (int b = sb; b < se; ++b) {
-      const PagesSeq s = pages_seq(p, b);
-      const long long w = pages_cost(segs, s);
-      if (begin < acc + w) { s_b = b; s_at = acc; break; }
-      acc += w;
+  int seq_b = 0;
+  long long seq_at = 0;         // where sequence seq_b begins in the dealt-out units
+  for (;; seq_b += 32) {
+    if (seq_b >= p.B) return;   // never, unless the lengths change under the call
+    const long long own = seq_cost(seq_b + lane);
+    long long upto = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
     }
+    const unsigned hit = __ballot_sync(0xffffffffu, begin < seq_at + upto);
+    if (hit) {
+      seq_b += __ffs(hit) - 1;
+      seq_at += __shfl_sync(0xffffffffu, upto - own, __ffs(hit) - 1);
+      break;
+    }
+    seq_at += __shfl_sync(0xffffffffu, upto, 31);
   }
-  __syncthreads();
-  volatile int* abort_flag = &s_abort;
-  int seq_b = s_b;
-  long long seq_at = s_at;      // where sequence seq_b begins in the dealt-out units
   PagesSeq seq = pages_seq(p, seq_b);
 
   // The piece of the share [at, end) that begins at `at`; false when nothing is left.  A segment's
@@ -217,7 +209,8 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
     while (at < end) {
       for (long long w; at >= seq_at + (w = pages_cost(segs, seq));) {
         seq_at += w;
-        seq = pages_seq(p, ++seq_b);
+        if (++seq_b >= p.B) return false;   // never, unless the lengths change under the call
+        seq = pages_seq(p, seq_b);
         while (seq.units == 0) {      // the next that has some, 32 at a look
           const unsigned some = __ballot_sync(0xffffffffu, seq_b + lane < p.B && pages_seq(p, seq_b + lane).units > 0);
           if (some) seq = pages_seq(p, seq_b += __ffs(some) - 1);
@@ -244,8 +237,9 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
   };
 
   int filled = 0, drained = 0;   // groups of this warp so far: a group's stage and phase
-  // lane l looks up unit l % U of group l / U of a batch of NB groups
-  struct Batch { int entry; float sk, log_v, inv_v; };
+  // lane l looks up unit l % U of group l / U of a batch of NB groups: the page ids two batches ahead, the
+  // scales one, so that neither load is waited for in the run of the groups
+  struct Batch { int entry; float2 scale; };
   auto look_up = [&](const PagesPiece& x, int k0) {
     const int u = x.first + ((k0 + lane / U) * kPgWarps + warp) * U + lane % U;
     int e = -1;
@@ -254,15 +248,12 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
     return e >= 0 && e < p.P ? e : -1;
   };
   auto look_up_scales = [&](const PagesPiece& x, Batch& q) {
-    float2 s = make_float2(1.f, 1.f);
-    if (q.entry >= 0) s = *reinterpret_cast<const float2*>(p.scales + ((long long)q.entry * p.G + x.gh) * 2);
-    q.sk = s.x;
-    q.log_v = __log2f(s.y);
-    q.inv_v = 1.f / s.y;
+    q.scale = make_float2(1.f, 1.f);
+    if (q.entry >= 0) q.scale = *reinterpret_cast<const float2*>(p.scales + ((long long)q.entry * p.G + x.gh) * 2);
   };
   // group k of the piece into the ring: lanes 0 .. U - 1 a unit each
-  auto fill = [&](const PagesPiece& x, const Batch& q, int k) {
-    const int entry = __shfl_sync(0xffffffffu, q.entry, (k % NB) * U + (lane % U));
+  auto fill = [&](const PagesPiece& x, int entries, int k) {
+    const int entry = __shfl_sync(0xffffffffu, entries, (k % NB) * U + (lane % U));
     const int u = x.first + (k * kPgWarps + warp) * U + lane;
     const bool on = lane < U && entry >= 0;
     const int n = __popc(__ballot_sync(0xffffffffu, on));
@@ -284,12 +275,20 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
 
   long long at = begin;
   PagesPiece cur;
-  Batch bat, bat_next;
+  Batch bat = {-1, make_float2(1.f, 1.f)}, bat_next = bat;
+  int entry_after = -1;
+  float key_scale = 1.f, log_v = 0.f, inv_v = 1.f;   // of `bat`
+  auto use_scales = [&]() {
+    key_scale = bat.scale.x;
+    log_v = __log2f(bat.scale.y);
+    inv_v = 1.f / bat.scale.y;
+  };
   uint4 q_raw[NT][D / 32];      // this lane's share of the query of column 8 nt + g: a run of D / 4
   // the loads that a piece begins with, in the order in which others wait for them
   auto open_piece = [&]() {
     bat.entry = look_up(cur, 0);
     bat_next.entry = look_up(cur, NB);
+    entry_after = look_up(cur, 2 * NB);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int c = nt * 8 + g;
@@ -297,9 +296,9 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) q_raw[nt][i] = c < cur.cols ? ld_cached(src + 8 * i) : make_uint4(0, 0, 0, 0);
     }
+    look_up_scales(cur, bat);     // before the copies: behind everybody's they would come last
     const int n = groups_of(cur);
-    for (int k = 0; k < kPgStages && k < n; ++k) fill(cur, bat, k);
-    look_up_scales(cur, bat);
+    for (int k = 0; k < kPgStages && k < n; ++k) fill(cur, bat.entry, k);
     look_up_scales(cur, bat_next);
   };
   bool have = next_piece(at, cur);
@@ -350,6 +349,7 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
         for (int j = 0; j < 4; ++j) o[i][nt][j] = 0.f;
     }
 
+    use_scales();
     const int groups = groups_of(cur);
     for (int k = 0; k < groups && ok; ++k) {
       const int stage = drained % kPgStages;
@@ -392,7 +392,7 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
 #pragma unroll
           for (int i = 0; i < U; ++i) {
             const uint32_t a[4] = {e4m3x2_to_half2(kf[i][0][c]), e4m3x2_to_half2(kf[i][1][c]),
-                                   e4m3x2_to_half2(kf[i][0][c] >> 16), e4m3x2_to_half2(kf[i][1][c] >> 16)};
+                                   e4m3x2_hi_to_half2(kf[i][0][c]), e4m3x2_hi_to_half2(kf[i][1][c])};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma_f16_16816(s[i][nt], a, qf[nt][c][0], qf[nt][c][1]);
           }
@@ -402,7 +402,7 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
         for (int nt = 0; nt < NT; ++nt) m_new[nt][0] = m_run[nt][0], m_new[nt][1] = m_run[nt][1];
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-          const float sk = __shfl_sync(0xffffffffu, bat.sk, src0 + i), lv = __shfl_sync(0xffffffffu, bat.log_v, src0 + i);
+          const float sk = __shfl_sync(0xffffffffu, key_scale, src0 + i), lv = __shfl_sync(0xffffffffu, log_v, src0 + i);
           bool seen[2] = {true, true};
           if (!kWhole) {
             const bool there = __shfl_sync(0xffffffffu, bat.entry, src0 + i) >= 0;
@@ -448,7 +448,7 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
           for (int j = 0; j < 2; ++j) zero[nt][j] = (m_run[nt][j] == -INFINITY ? 0.f : m_run[nt][j]) - kPgLift;
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-          const float inv_v = __shfl_sync(0xffffffffu, bat.inv_v, src0 + i);
+          const float inv = __shfl_sync(0xffffffffu, inv_v, src0 + i);
           uint32_t pb[NT][2];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
@@ -456,7 +456,7 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) pr[j] = ex2(s[i][nt][j] - zero[nt][j & 1]);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) l_run[nt][j] = fmaf(pr[j] + pr[j + 2], inv_v, l_run[nt][j]);
+            for (int j = 0; j < 2; ++j) l_run[nt][j] = fmaf(pr[j] + pr[j + 2], inv, l_run[nt][j]);
             pb[nt][0] = movmatrix_trans(pack_half2(pr[0], pr[1]));
             pb[nt][1] = movmatrix_trans(pack_half2(pr[2], pr[3]));
           }
@@ -482,7 +482,7 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
           for (int c = 0; c < KS; ++c) {
             const uint32_t sel = (c & 1) ? 0x7362u : 0x5140u;
             const uint32_t x = prmt(vf[0][c >> 1], vf[1][c >> 1], sel), y = prmt(vf[2][c >> 1], vf[3][c >> 1], sel);
-            const uint32_t a[4] = {e4m3x2_to_half2(x), e4m3x2_to_half2(x >> 16), e4m3x2_to_half2(y), e4m3x2_to_half2(y >> 16)};
+            const uint32_t a[4] = {e4m3x2_to_half2(x), e4m3x2_hi_to_half2(x), e4m3x2_to_half2(y), e4m3x2_hi_to_half2(y)};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma_f16_16816(o[c][nt], a, pb[nt][0], pb[nt][1]);
           }
@@ -492,11 +492,13 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
       // ---- the stage is read: the group kPgStages on takes it ----
       __syncwarp();
       const int kf_ = k + kPgStages;
-      if (kf_ < groups) fill(cur, kf_ / NB == k / NB ? bat : bat_next, kf_);
+      if (kf_ < groups) fill(cur, kf_ / NB == k / NB ? bat.entry : bat_next.entry, kf_);
       if ((k + 1) % NB == 0) {
         bat = bat_next;
-        bat_next.entry = look_up(cur, k + 1 + NB);
+        use_scales();
+        bat_next.entry = entry_after;
         look_up_scales(cur, bat_next);
+        entry_after = look_up(cur, k + 1 + 2 * NB);
       }
     }
 

@@ -132,7 +132,8 @@ struct PtWalk {
         j = 0;
         if (++g >= p.G) {
           g = 0;
-          seq = pt_seq(p, ++b);
+          if (++b >= p.B) return false;   // never, unless the lengths change under the call
+          seq = pt_seq(p, b);
           while (seq.blocks == 0) {
             // the next sequence with rows, 32 at a look
             const int lane = threadIdx.x & 31;
@@ -263,8 +264,8 @@ __device__ __forceinline__ float score_factor(float row, uint32_t key_scale) {
 }
 // Sixteen codes -> sixteen halves.
 __device__ __forceinline__ void halves16(const uint4& c, uint4& lo, uint4& hi) {
-  lo = make_uint4(e4m3x2_to_half2(c.x), e4m3x2_to_half2(c.x >> 16), e4m3x2_to_half2(c.y), e4m3x2_to_half2(c.y >> 16));
-  hi = make_uint4(e4m3x2_to_half2(c.z), e4m3x2_to_half2(c.z >> 16), e4m3x2_to_half2(c.w), e4m3x2_to_half2(c.w >> 16));
+  lo = make_uint4(e4m3x2_to_half2(c.x), e4m3x2_hi_to_half2(c.x), e4m3x2_to_half2(c.y), e4m3x2_hi_to_half2(c.y));
+  hi = make_uint4(e4m3x2_to_half2(c.z), e4m3x2_hi_to_half2(c.z), e4m3x2_to_half2(c.w), e4m3x2_hi_to_half2(c.w));
 }
 
 template <int D>
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
   for (int b0 = sb; b0 < se; b0 += 32) mine += costs(seq_at(b0 + lane));
   mine = warp_sum_ll(mine) * p.G;
   if (lane == 0) s_sum[warp] = mine;
-  if (tid == 0) { s_nan = 0; p.records[blockIdx.x].pieces = 0; }
+  if (tid == 0) { s_nan = s_b = s_g = s_j = 0; s_at = 0; p.records[blockIdx.x].pieces = 0; }
   __syncthreads();
   long long before = 0, total = 0;
   for (int w = 0; w < kWarps; ++w) {

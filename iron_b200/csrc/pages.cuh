@@ -26,6 +26,12 @@ __device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t codes) {
   asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(codes));
   return r;
 }
+// The same of a register's upper two codes: named as a half register, so that no shift is needed.
+__device__ __forceinline__ uint32_t e4m3x2_hi_to_half2(uint32_t codes) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(codes));
+  return r;
+}
 __device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t codes) {
   const uint32_t h = e4m3x2_to_half2(codes);
   float2 f;
