@@ -31,10 +31,12 @@
 //
 // Over ragged rows (row_start) the kernel takes the sequences that bring one row and passes the others.
 //
-// Measured (32 heads over 8): 64 sequences of 2048, heads of 64: 33.3 us (135 MB, 4.0 TB/s, 62 % of a plain
-// copy's rate); one of 120,001, heads of 128: 52 us (4.7 TB/s, 72 %); 128 of 3 to 8191, over 4: 37.8 us (3.7
-// TB/s); one of 500: 9.4 us.  What bounds it is the instructions between the bytes, not the bytes: 44 % of the
-// issue slots at 11 warps an SM, each unit a chain of conversions, products and exponentials.
+// Measured (32 heads over 8): 64 sequences of 2048, heads of 64: 31.9 us (135 MB, 4.2 TB/s, 65 % of a plain
+// copy's rate); one of 120,001, heads of 128: 50.8 us (4.8 TB/s, 74 %); 128 of 3 to 8191, over 4, that hold
+// 141 MB: 36.4 us (3.9 TB/s), 550 MB: 102 us (5.4 TB/s, 83 %); one of 500: 8.9 us.  A long call is bound by
+// bytes; in a short one some 13,000 clocks go by before a CTA's first product (share, page ids, scales, copies),
+// and each unit is a chain of conversions, products and exponentials (200 instructions at heads of 64, half
+// of them on the integer pipe).
 #include <type_traits>
 
 #include "common.cuh"
@@ -47,13 +49,13 @@ namespace iron {
 constexpr int kPgWarps = 4;
 constexpr int kPgThreads = kPgWarps * 32;
 // CTAs an SM: what the registers of one or of two groups of eight columns allow without spilling.  (Two for
-// one group: 64 x 2048 35.7 us for 33.3, one long sequence 48.7 for 52.)
+// one group: 64 x 2048 33.9 us for 31.9, 200 of 1 to 3000 76 for 67, one long sequence 48.8 for 50.8.)
 constexpr int pg_ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 constexpr int kPgCtas = kSMs * pg_ctas_per_sm(1);
 constexpr int kPgUnit = 16;                 // tokens
 constexpr int kPgStages = 2;                // of a warp's ring; a stage holds kGroup units
 // Units a segment costs beside its own: its queries and the meeting of its warps.  128 sequences of 3 to
-// 8191 with 8, 16, 24 and 40: 57, 41.7, 37.8 and 40.1 us; even lengths do not care.
+// 8191 that hold 141 MB with 8, 16, 24 and 40: 57, 41.7, 37.8 and 40.1 us; even lengths do not care.
 constexpr int kPgSegCost = 24;
 constexpr float kPgLift = 10.f;             // log2 of what probabilities are held times
 
@@ -709,7 +711,7 @@ static int launch_pages(PagesParams p, cudaStream_t stream) {
 
 template <int D>
 static int launch_pages_cols(const PagesParams& p, int cols, cudaStream_t stream) {
-  // one group of eight columns where the heads of a KV head fit it (64 x 2048 with two: 41.9 us for 33.3)
+  // one group of eight columns where the heads of a KV head fit it (64 x 2048 with two: 41.9 us for 33.3, before the look-ups were moved ahead)
   return cols <= 8 ? launch_pages<D, 1>(p, stream) : launch_pages<D, 2>(p, stream);
 }
 

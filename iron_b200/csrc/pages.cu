@@ -330,7 +330,8 @@ __global__ void __launch_bounds__(kWriteThreads, 4) rope_kv_pages_kernel(const W
     const long long total = (long long)p.rows * p.H * kPieces;
     for (long long i = (long long)(blockIdx.x - p.kv_blocks) * kWriteThreads + tid; i < total;
          i += (long long)(gridDim.x - p.kv_blocks) * kWriteThreads) {
-      const int piece = (int)(i % kPieces), h = (int)(i / kPieces % p.H), r = (int)(i / kPieces / p.H);
+      const int r = (int)div_ll(i, p.H * kPieces), of_row = (int)(i - (long long)r * (p.H * kPieces));
+      const int piece = of_row % kPieces, h = of_row / kPieces;
       float a[8], b[8];
       load_turned<D>(p, r, h, piece * 8, true, a, b);
       __nv_bfloat16* dst = p.q_out + ((size_t)r * p.H + h) * D + piece * 8;
