@@ -33,7 +33,7 @@
 // there, 560 for the maximum, 1250 for the weights, the rest handing over) where exponentials alone would
 // take 1024, the exponentials' pipe is 41 % busy and the tensor pipe 41 %; registers allow no third
 // group of warps to fill it.  Narrow items (few columns) wait for the converters, 5000 clocks a tile; a
-// call has some 14,000 clocks before its first tile and 4000 after an item's last.
+// call has 12,000 to 14,000 clocks before its first tile and 4000 after an item's last.
 //
 // Every mbarrier wait is bounded; a wait that gives up sets the abort flag, every role unwinds,
 // tensor memory is freed and the status word receives IRON_ERR_TIMEOUT.
@@ -295,6 +295,23 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
   constexpr int kWarps = kPtThreads / 32;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+  // the barriers are set up by the warp that has no role, before and beside what the others look up
+  if (tid == kPtThreads - 32) {
+    for (int s = 0; s < Cfg::kStages; ++s) {
+      mbar_init(k_full + s, 128); mbar_init(k_empty + s, 2); mbar_init(v_full + s, 128); mbar_init(v_empty + s, 2);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full + i, 128);
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(s_full + 2 * i + k, 1); mbar_init(p_full + 2 * i + k, 128); mbar_init(o_full + 2 * i + k, 1);
+      }
+      mbar_init(o_free + i, 128);
+    }
+    for (int s = 0; s < kPtSlots; ++s) { mbar_init(item_full + s, 1); mbar_init(item_empty + s, kPtRoles); }
+    for (int s = 0; s < kPtScales; ++s) mbar_init(scale_full + s, 4);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   pdl_launch();
   pdl_wait();
   // ---- where this CTA's share begins: a warp sums a stretch of the sequences, 32 at a look ----
@@ -338,11 +355,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
   if (lane == 0) s_sum[warp] = mine;
   if (tid == 0) { s_nan = s_b = s_g = s_j = 0; s_at = 0; p.records[blockIdx.x].pieces = 0; }
   __syncthreads();
-  long long before = 0, total = 0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += s_sum[w];
-    total += s_sum[w];
-  }
+  const long long warp_sum = lane < kWarps ? s_sum[lane] : 0, upto_warp = upto_lane(warp_sum);
+  const long long before = __shfl_sync(0xffffffffu, upto_warp - warp_sum, warp), total = __shfl_sync(0xffffffffu, upto_warp, 31);
   const long long share = max((long long)kPtMinShare, div_ll(total + gridDim.x - 1, gridDim.x));
   const long long begin = (long long)blockIdx.x * share, end = min(begin + share, total);
   if (begin >= end) return;
@@ -356,7 +370,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
       const int l = __ffs(hit) - 1;
       const long long one = __shfl_sync(0xffffffffu, own, l);
       acc += __shfl_sync(0xffffffffu, upto, l) - one * p.G;
-      const int g = (int)((begin - acc) / one);
+      const int g = (int)(one >> 31 ? (begin - acc) / one : div_ll(begin - acc, (int)one));
       acc += one * g;
       s = pt_seq(p, b0 + l);
       for (int j0 = 0; j0 < s.blocks; j0 += 32) {
@@ -373,22 +387,6 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
       }
       break;
     }
-  }
-  if (tid == 0) {
-    for (int s = 0; s < Cfg::kStages; ++s) {
-      mbar_init(k_full + s, 128); mbar_init(k_empty + s, 2); mbar_init(v_full + s, 128); mbar_init(v_empty + s, 2);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(q_full + i, 128);
-      for (int k = 0; k < 2; ++k) {
-        mbar_init(s_full + 2 * i + k, 1); mbar_init(p_full + 2 * i + k, 128); mbar_init(o_full + 2 * i + k, 1);
-      }
-      mbar_init(o_free + i, 128);
-    }
-    for (int s = 0; s < kPtSlots; ++s) { mbar_init(item_full + s, 1); mbar_init(item_empty + s, kPtRoles); }
-    for (int s = 0; s < kPtScales; ++s) mbar_init(scale_full + s, 4);
-    *abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
