@@ -133,7 +133,8 @@ __global__ void __launch_bounds__(kStepThreads) page_step_kernel(
         const int pi = pos >> log_page, held = (len + page - 1) >> log_page;
         const int entry = pi < held ? tables[(size_t)b * width + pi]
                                     : pages[(int)(((long long)head + first_taken[b] + (pi - held)) % P)];
-        slot = entry * page + (pos & (page - 1));
+        // an id that is no page's has no slots: decided before the product, which could wrap into the pool
+        if ((unsigned)entry < (unsigned)P) slot = entry * page + (pos & (page - 1));
       }
     }
     slots[r] = slot;

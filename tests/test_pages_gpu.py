@@ -604,3 +604,67 @@ def test_a_tensor_of_another_kind_of_memory_is_refused():
         K.mha_decode_pages(q, pool, scales, t.cpu(), l)
     with pytest.raises(ValueError):
         K.mha_decode_pages(q, pool[:, :, :, ::2], scales, t, l)
+
+
+# ---------------------------------------------------------------------------- bad page ids
+def guarded(x):
+    """``x`` as int32 inside a larger buffer: (the tensor, a check that what lies around it is as it was)."""
+    x = np.asarray(x)
+    buffer = torch.full((x.size + 128,), 0x5A5A5A5A, dtype=I32, device="cuda")
+    inner = buffer[64:64 + x.size].view(x.shape)
+    inner.copy_(ints(x))
+    return inner, lambda: bool((buffer[:64] == 0x5A5A5A5A).all() and (buffer[64 + x.size:] == 0x5A5A5A5A).all())
+
+
+@pytest.mark.parametrize("page", [16, 256])
+@pytest.mark.parametrize("bad", [-1, 12, 1 << 28, (1 << 28) + 5, 1 << 30, -(1 << 28), (1 << 24) + 3, -(1 << 31), (1 << 31) - 1])
+def test_page_ids_outside_the_pool_give_no_slots(page, bad):
+    """Held or taken from the ring, an id that is no page's is never turned into a slot, not even where
+    its product with the page size wraps into the pool: the rows' slots are -1 and a write changes
+    nothing but the pages of the others."""
+    from iron_b200 import kernels as K
+
+    P, H, G, D = 12, 2, 1, 64
+    t, t_ok = guarded([[bad, 1], [-1, -1], [7, -1], [2, bad]])
+    l, n = ints([5, 0, 3, page]), ints([4, 3, 2, 1])
+    p, p_ok = guarded([bad] + [9] * (P - 1))
+    slots, s_ok = guarded(np.zeros(12))
+    positions, pos_ok = guarded(np.zeros(12))
+    K.page_step(t, l, n, p, ints([0, P, 0, 0]), page_size=page, rows=12, lengths_out=l, slots=slots, positions=positions)
+    assert slots.tolist() == [-1] * 7 + [7 * page + 3, 7 * page + 4, 9 * page, -1, -1]
+    assert positions.tolist() == [5, 6, 7, 8, 0, 1, 2, 3, 4, page, 0, 0] and l.tolist() == [9, 3, 5, page + 1]
+    assert t.tolist() == [[bad, 1], [bad, -1], [7, -1], [2, 9]]
+    assert t_ok() and p_ok() and s_ok() and pos_ok()
+    pool, scales = R.cache(P, G, page, D, 1)
+    before, scales_before = pool.view(torch.uint8).clone(), scales.clone()
+    qkv, angles = queries(12, H + 2 * G, D, 2).reshape(12, -1), torch.ones((8, D), dtype=BF16, device="cuda")
+    K.rope_kv_pages(qkv, angles, torch.empty((12, H, D), dtype=BF16, device="cuda"), pool, scales, slots, positions, H=H, G=G, D=D)
+    others = [i for i in range(P) if i not in (7, 9)]
+    assert torch.equal(pool.view(torch.uint8)[others], before[others]) and torch.equal(scales[others], scales_before[others])
+    assert not torch.equal(pool.view(torch.uint8)[7], before[7]) and not torch.equal(pool.view(torch.uint8)[9], before[9])
+
+
+@pytest.mark.parametrize("head, count", [(-7, 99), (2, -4), (1 << 30, 3), (-(1 << 31), (1 << 31) - 1)])
+def test_a_ring_that_says_nonsense_serves_inside_its_buffers(head, count):
+    """A ring's head and count outside their ranges, bad ids in it, lengths below zero and past the
+    table: requests are served, nothing around the buffers changes, and every slot is -1 or a page's."""
+    from iron_b200 import kernels as K
+
+    B, width, page, P, rows = 6, 4, 16, 5, 90
+    t, t_ok = guarded(np.full((B, width), 1 << 29))
+    l, l_ok = guarded([5, -4, 1 << 30, 20, 0, (1 << 31) - 1])
+    p, p_ok = guarded([-9, 1 << 28, 3, 1 << 30, 4])
+    outs = [guarded(np.zeros(k)) for k in (rows, rows, B + 1, 4)]
+    slots, positions, row_start, ring = (o[0] for o in outs)
+    ring.copy_(torch.tensor([head, count, 0, 0], dtype=I32))
+    K.page_step(t, l, ints([20, -1, 20, 3, 9, 1]), p, ring, page_size=page, rows=rows, lengths_out=l, ring_out=ring,
+                slots=slots, positions=positions, row_start=row_start)
+    assert t_ok() and l_ok() and p_ok() and all(ok() for _, ok in outs)
+    assert row_start.tolist() == [0, 20, 20, 40, 43, 52, 53]
+    got = slots.tolist()
+    assert all(s == -1 or 0 <= s < P * page for s in got) and got[53:] == [-1] * 37
+    assert got[:11] == [-1] * 11                             # the request's first page is 1 << 29, which wraps to 0
+    free = max(0, min(count, P))
+    assert l.tolist() == [25 if free >= 1 else 5, 0, 1 << 30, 23, 9 if free >= 2 else 0, (1 << 31) - 1]
+    assert 0 <= ring[0].item() < P and ring.tolist()[1:] == [free - min(free, 2), 2 if free else 4, 53]
+    assert any(s >= 0 for s in got) == (free > 0)            # one of the ring's next two ids is a page's
