@@ -617,7 +617,8 @@ int iron_decode_step_bf16(const void* const* layer_ptrs, const void* maps, int L
  * offset; -1 past the last row, for a request that was not served, and where the page id is not in
  * 0 .. P - 1) and positions;
  * lengths_out (may be lengths) and ring_out = (head, count, requests not served, rows asked for;
- * may be ring).  At most iron_page_step_max_requests() requests. */
+ * may be ring).  At most iron_page_step_max_requests() requests; P * page_size and width * page_size
+ * stay below 2^31 (slots and positions are 32-bit). */
 int iron_page_step_max_requests(void);
 int iron_page_step(int* tables, int width, const int* lengths, const int* new_tokens, int B,
                    int* pages, int P, const int* ring, int page_size, int rows,

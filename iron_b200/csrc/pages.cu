@@ -390,7 +390,8 @@ extern "C" int iron_page_step(int* tables, int width, const int* lengths, const 
                               int* slots, int* positions, int* row_start, iron_stream_t stream) {
   const int log_page = log2_page(page_size);
   if (B < 0 || B > kMaxRequests || width <= 0 || P <= 0 || rows < 0 || log_page < 0) return IRON_ERR_SHAPE;
-  if ((long long)P * page_size > 0x7fffffffll) return IRON_ERR_SHAPE;   // slots are 32-bit
+  // slots and positions are 32-bit
+  if ((long long)P * page_size > 0x7fffffffll || (long long)width * page_size > 0x7fffffffll) return IRON_ERR_SHAPE;
   if (!ring || !ring_out || !row_start || !pages) return IRON_ERR_SHAPE;
   if (B > 0 && (!tables || !lengths || !new_tokens || !lengths_out)) return IRON_ERR_SHAPE;
   if (rows > 0 && (!slots || !positions)) return IRON_ERR_SHAPE;

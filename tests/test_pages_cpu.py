@@ -144,3 +144,11 @@ def test_the_plain_codes_are_torchs():
     want = torch.from_numpy(x).float().to(F8).double().numpy()
     assert np.array_equal(R.e4m3(x.astype(np.float32).astype(np.float64)), want)
     assert [R.scale_of(np.array([v])) for v in (448.0, 449.0, 0.0, 1.75, 1.76)] == [1, 2, 2.0 ** -60, 2.0 ** -8, 2.0 ** -7]
+
+
+@pytest.mark.parametrize("page", [16, 64, 256])
+def test_page_step_refuses_tables_whose_tokens_pass_32_bits(page):
+    """Positions are 32-bit: a table wide enough for more tokens is refused before any launch."""
+    lib, a, wide = _lib.load(), 16, (1 << 31) // page
+    step = lambda width: lib.iron_page_step(a, width, a, a, 1, a, 4, a, page, 1, a, a, a, a, a, None)  # noqa: E731
+    assert step(wide) == step((1 << 31) - 1) == -1
