@@ -107,7 +107,7 @@ __device__ __forceinline__ void pt_block(const PagesParams& p, const PtSeq& s, i
   x.any_lo = p.window >= 0 ? max(0, first - p.window) : 0;
   x.all_lo = p.window >= 0 ? last - p.window : 0;
   x.any_hi = p.causal ? max(0, min(s.len, last + 1)) : s.len;
-  x.all_hi = p.causal ? min(s.len, first + 1) : s.len;
+  x.all_hi = p.causal ? max(0, min(s.len, first + 1)) : s.len;
   x.tile0 = x.any_lo / kPtKeys;
   x.tiles = max(1, (x.any_hi + kPtKeys - 1) / kPtKeys - x.tile0);
 }
@@ -585,7 +585,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
     float2 scale = make_float2(1.f, 0.f);
     auto unit_of = [&]() {
       const bool there = entry >= 0 && entry < p.P;
-      // an absent page: its scores are -inf through the logarithm, its share of the sum nothing
+      // an absent page: finite scores are -inf through the logarithm, its share of the sum nothing; an inverse of 0 marks it
       scale = make_float2(1.f, 0.f);
       if (!values && there && lane < 2)
         scale = *reinterpret_cast<const float2*>(p.scales + ((long long)entry * p.G + it.gh) * 2);
@@ -695,6 +695,10 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
       const int e = min(max((int)(__float_as_uint(mx) >> 23), 15), 254);
       const float up = __uint_as_float((uint32_t)(268 - e) << 23);
       me.factor = p.scale_log2 / up;
+      // The logarithm of an absent page's scale masks finite scores, but a query that is not finite times the
+      // page's zeros is NaN.  Where a row of this warp has one, no key counts as seen by all (the bound is
+      // kept as its complement), and every step takes the masks below.
+      if (__any_sync(0xffffffffu, mx == INFINITY || mx != mx)) it.all_hi = ~it.all_hi;
 #pragma unroll
       for (int k = 0; k < D / 8; ++k) {
         float f[8];
@@ -746,6 +750,14 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
 #pragma unroll
           for (int k = 0; k < 64; ++k)
             if (key0 + k >= hi_key || key0 + k < lo_key) v[k] = 0xff800000u;   // this column does not see the key
+          // absent pages (an inverse of 0), under queries that are not finite; 1.6 % of the eight chunks' time
+          if (__builtin_expect(it.all_hi < 0, 0)) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (f[q].z == 0)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v[16 * q + k] = 0xff800000u;
+          }
         }
         // ---- the maximum ----
         float mx = -INFINITY;
@@ -833,7 +845,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
           const int from = max(was.lo_key, (done.tile0 + done.t_lo) * kPtKeys), to = min(was.hi_key, (done.tile0 + done.t_hi) * kPtKeys);
           for (int key = max(from, 0); key < to; ++key) {
             const int k0 = key / kPtKeys * kPtKeys;
-            if (k0 >= done.all_lo && k0 + kPtKeys <= done.all_hi) { key = k0 + kPtKeys - 1; continue; }
+            if (k0 >= done.all_lo && k0 + kPtKeys <= max(done.all_hi, ~done.all_hi)) { key = k0 + kPtKeys - 1; continue; }
             const int e = p.tables[(long long)done.b * p.width + (key >> p.log_page)];
             if (e < 0 || e >= p.P) continue;
             const long long block = ((long long)e * p.G + done.gh) * 2 + 1;

@@ -668,3 +668,44 @@ def test_a_ring_that_says_nonsense_serves_inside_its_buffers(head, count):
     assert l.tolist() == [25 if free >= 1 else 5, 0, 1 << 30, 23, 9 if free >= 2 else 0, (1 << 31) - 1]
     assert 0 <= ring[0].item() < P and ring.tolist()[1:] == [free - min(free, 2), 2 if free else 4, 53]
     assert any(s >= 0 for s in got) == (free > 0)            # one of the ring's next two ids is a page's
+
+
+# ---------------------------------------------------------------------------- queries that are not finite
+@pytest.mark.parametrize("form", ["decode", "prompt", "single rows among others"])
+@pytest.mark.parametrize("D, page", [(64, 16), (128, 64), (64, 256)])
+@pytest.mark.parametrize("kw", [dict(), dict(window=70), dict(causal=False)], ids=str)
+def test_infinite_and_nan_queries_over_present_and_absent_pages(form, D, page, kw):
+    """An absent token is not there for a query of any value: rows all of whose present scores are
+    -infinity, and rows that see no present token, are zeros; a NaN or +infinity in a score is NaN."""
+    from iron_b200 import kernels as K
+
+    if form == "decode" and "causal" in kw:
+        kw = dict(window=0)                                  # a decode step has no mask to drop
+    H, G = 8, 2
+    lengths, new = [700, 400, 300, 40], [150, 130, 200, 5]
+    if form != "prompt":
+        new = [1, 1, 1, 1]
+    if form == "single rows among others":
+        lengths, new = lengths + [9] * 20, new + [0] * 19 + [3]
+    tables, P = R.tables_for(lengths, page, 1)
+    pool, scales = R.cache(P, G, page, D, 3)
+    poison(pool, scales, tables, lengths, page)
+    pool[:, :, 0, :, 7] = torch.where(torch.isnan(pool[:, :, 0, :, 7].float()), 0.0, 2.0).to(F8)   # every key's element 7 is there
+    tables[0, ::3] = -1
+    tables[1, :] = P + 5                                     # a request none of whose pages is there
+    start = np.concatenate(([0], np.cumsum(new)))
+    q, inf, nan = queries(int(start[-1]), H, D, 5), math.inf, math.nan
+    for b in range(4):
+        for r in {start[b], (start[b] + start[b + 1]) // 2, start[b + 1] - 1}:
+            q[r, 0, 7], q[r, 1, 7], q[r, 3, 2], q[r, 5, :], q[r, 6, 7] = -inf, inf, nan, -inf, -inf
+            q[r, 6, 3] = 3e38
+    t, l = ints(tables), ints(lengths)
+    if form == "decode":
+        out = K.mha_decode_pages(q, pool, scales, t, l, **kw)
+    else:
+        out = K.mha_prefill_pages(q, pool, scales, t, l, ints(start), **kw)
+    want, size = R.attention(q, pool, scales, t, lengths, start, **kw)
+    zero = (want[start[0]:start[1]] == 0).all(-1)
+    assert zero.any() and torch.isnan(want).any() and (want[start[1]:start[2]] == 0).all()
+    check_attention(out, want, size)
+    assert (out[start[1]:start[2]] == 0).all()
