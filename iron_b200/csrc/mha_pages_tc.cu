@@ -312,7 +312,6 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  pdl_launch();
   pdl_wait();
   // ---- where this CTA's share begins: a warp sums a stretch of the sequences, 32 at a look ----
   const int per_warp = (p.B + kWarps - 1) / kWarps;
@@ -398,6 +397,9 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = *tmem_slot;
+  // Successors may start only now: one that takes tensor memory before its own wait must not find a CTA
+  // here that still asks for its columns, or each would wait for the other.
+  pdl_launch();
 
   bool ok = true;
   // The next item, from the ring that warp 18 fills; `take` copies what the role needs of it.
