@@ -643,7 +643,10 @@ int iron_rope_kv_pages_e4m3(const void* qkv, long long pitch, const void* angles
  * zeros, and so does a query all of whose scores are -infinity.  A length past width * page counts
  * as that.  `workspace` (iron_mha_pages_workspace_bytes(D, 0) bytes, 16-byte aligned) holds the call's
  * partial results; it needs no clearing, and two calls that may overlap need one each.  `status`
- * (may be NULL) receives IRON_ERR_TIMEOUT when a bounded wait of the pipeline gives up. */
+ * receives IRON_ERR_TIMEOUT when a bounded wait of the pipeline gives up (the output is then not
+ * complete) and keeps it until the caller clears it; where it is NULL, the library's own word of the
+ * current device does, which iron_mha_pages_status_word() names (NULL without a device). */
+int* iron_mha_pages_status_word(void);
 long long iron_mha_pages_workspace_bytes(int D, int prompt);
 int iron_mha_decode_pages_bf16(const void* q, const void* pool, const float* scales, int P,
                                int page_size, const int* tables, int width, const int* lengths,

@@ -109,6 +109,7 @@ SIGNATURES: dict[str, tuple] = {
     "iron_page_step_max_requests": (_I, []),
     "iron_page_step": (_I, [_P, _I, _P, _P, _I, _P, _I, _P, _I, _I, _P, _P, _P, _P, _P, _P]),
     "iron_rope_kv_pages_e4m3": (_I, [_P, _L, _P, _P, _P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _P]),
+    "iron_mha_pages_status_word": (_P, []),
     "iron_mha_pages_workspace_bytes": (_L, [_I, _I]),
     "iron_mha_decode_pages_bf16": (
         _I,

@@ -657,6 +657,22 @@ __global__ void __launch_bounds__(kFoldWarps * 32) mha_pages_fold_kernel(const P
   }
 }
 
+// What a call without a status word of its own reports to: one word a device, the library's.
+__device__ int g_pages_status;
+static int* pages_status_word() {
+  static std::atomic<int*> known[64];
+  const int dev = current_device();
+  if (dev < 0) return nullptr;
+  int* word = known[dev].load(std::memory_order_acquire);
+  if (!word) {
+    void* at = nullptr;
+    if (cudaGetSymbolAddress(&at, g_pages_status) != cudaSuccess) return nullptr;
+    word = (int*)at;
+    known[dev].store(word, std::memory_order_release);
+  }
+  return word;
+}
+
 typedef CUresult (*PgEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -723,6 +739,8 @@ static int launch_decode(const PagesParams& p, int D, cudaStream_t stream) {
 
 using namespace iron;
 
+extern "C" int* iron_mha_pages_status_word(void) { return pages_status_word(); }
+
 extern "C" long long iron_mha_pages_workspace_bytes(int D, int prompt) {
   if (D != 64 && D != 128) return 0;
   const long long partial = 16ll * D + 32;
@@ -769,7 +787,7 @@ extern "C" int iron_mha_decode_pages_bf16(const void* q, const void* pool, const
   const int rc = pages_args(p, q, pool, scales, P, page_size, tables, width, lengths, nullptr, B, B, H, G, D, 1, window,
                             scale, workspace, workspace_bytes, out);
   if (rc) return rc == 1 ? IRON_OK : rc;
-  p.status = status;
+  p.status = status ? status : pages_status_word();
   return launch_decode(p, D, (cudaStream_t)stream);
 }
 
@@ -782,7 +800,7 @@ extern "C" int iron_mha_prefill_pages_bf16(const void* q, const void* pool, cons
                             causal, window, scale, workspace, workspace_bytes, out);
   if (rc) return rc == 1 ? IRON_OK : rc;
   if (!row_start) return IRON_ERR_SHAPE;
-  p.status = status;
+  p.status = status ? status : pages_status_word();
   // A sequence of one row fills hg of the ragged kernel's 128 lanes, the decode kernel's eight columns
   // well.  32 heads over 8 of 128, pages of 64, without and with the split: 256 x 1 row on 300 tokens
   // 187 and 67 us, 64 x 1 on 3000 185 and 80, 16 x 1 on 300 27.6 and 21.5; where no sequence has one row

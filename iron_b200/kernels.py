@@ -690,6 +690,28 @@ def pages_workspace(D: int, prompt: bool = False, device=None) -> torch.Tensor:
     return torch.empty(n, dtype=torch.uint8, device=device or "cuda")
 
 
+class _DeviceWord:
+    """One int32 of device memory that the library owns, as ``torch.as_tensor`` takes it."""
+
+    def __init__(self, address: int):
+        self.__cuda_array_interface__ = dict(shape=(1,), typestr="<i4", data=(address, False), version=2)
+
+
+_PAGES_STATUS: dict[int, torch.Tensor] = {}
+
+
+def pages_status(device=None) -> torch.Tensor:
+    """The device word (one int32) in which paged attention calls without a ``status`` of their own
+    report a wait that gave up (``IRON_ERR_TIMEOUT``: the call's output is not complete); it keeps the
+    report until it is cleared (``zero_()``).  Read it where the program meets the device anyway."""
+    dev = torch.cuda.current_device() if device is None else torch.device(device).index
+    dev = torch.cuda.current_device() if dev is None else dev
+    if dev not in _PAGES_STATUS:
+        with torch.cuda.device(dev):
+            _PAGES_STATUS[dev] = torch.as_tensor(_DeviceWord(_lib.load().iron_mha_pages_status_word()), device=f"cuda:{dev}")
+    return _PAGES_STATUS[dev]
+
+
 def _window(window) -> int:
     """A window as the C entries take it: -1 for none, and what passes 32 bits leaves nothing out either."""
     return -1 if window is None else min(int(window), 2**31 - 1)
@@ -727,7 +749,7 @@ def mha_decode_pages(Q, pool, scales, tables, lengths, out=None, *, window=None,
 
     ``window`` keeps the keys within that many positions of the last.  ``workspace``:
     ``pages_workspace``'s buffer, allocated for the call when not given; ``status``: an int32 word
-    that receives ``IRON_ERR_TIMEOUT`` when a bounded wait gives up."""
+    that receives ``IRON_ERR_TIMEOUT`` when a bounded wait gives up (``pages_status``'s when not given)."""
     if Q.shape[:1] != lengths.shape:
         raise ValueError(f"Q {tuple(Q.shape)} is not one query for each of {tuple(lengths.shape)} requests")
     P, G, page, D, out, workspace, stream = _pages_attention(Q, pool, scales, tables, lengths, out, workspace)

@@ -152,3 +152,8 @@ def test_page_step_refuses_tables_whose_tokens_pass_32_bits(page):
     lib, a, wide = _lib.load(), 16, (1 << 31) // page
     step = lambda width: lib.iron_page_step(a, width, a, a, 1, a, 4, a, page, 1, a, a, a, a, a, None)  # noqa: E731
     assert step(wide) == step((1 << 31) - 1) == -1
+
+
+def test_without_a_device_there_is_no_status_word():
+    if not torch.cuda.is_available():
+        assert _lib.load().iron_mha_pages_status_word() is None

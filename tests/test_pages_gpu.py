@@ -709,3 +709,27 @@ def test_infinite_and_nan_queries_over_present_and_absent_pages(form, D, page, k
     assert zero.any() and torch.isnan(want).any() and (want[start[1]:start[2]] == 0).all()
     check_attention(out, want, size)
     assert (out[start[1]:start[2]] == 0).all()
+
+
+# ---------------------------------------------------------------------------- status words
+@pytest.mark.parametrize("prompt", [False, True])
+def test_status_words(prompt):
+    """A wait that gives up is reported to the call's word, or to the device's own, never to nobody; calls
+    that end well touch neither, and what a word holds stays until it is cleared.  (No wait of these
+    kernels can be made to give up without breaking one, so the report itself is not run here.)"""
+    from iron_b200 import kernels as K
+
+    H, G, D, page, lengths = 4, 2, 64, 16, [40, 3]
+    tables, P = R.tables_for(lengths, page, 1)
+    pool, scales = R.cache(P, G, page, D, 2)
+    q, t, l = queries(2, H, D, 1), ints(tables), ints(lengths)
+    call = (lambda **kw: K.mha_prefill_pages(q, pool, scales, t, l, ints([0, 1, 2]), **kw)) if prompt else (
+        lambda **kw: K.mha_decode_pages(q, pool, scales, t, l, **kw))
+    word = K.pages_status()
+    assert word.dtype is I32 and word.shape == (1,) and word.is_cuda and int(word) == 0
+    assert K.pages_status(q.device).data_ptr() == K.pages_status("cuda").data_ptr() == word.data_ptr()
+    own = torch.zeros(1, dtype=I32, device="cuda")
+    for value in (0, -6):
+        own.fill_(value), word.fill_(value)
+        assert torch.equal(call(), call(status=own)) and int(own) == int(word) == value
+    word.zero_()
