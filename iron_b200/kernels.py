@@ -717,7 +717,7 @@ def _window(window) -> int:
     return -1 if window is None else min(int(window), 2**31 - 1)
 
 
-def _pages_attention(Q, pool, scales, tables, lengths, out, workspace, row_start=None):
+def _pages_attention(Q, pool, scales, tables, lengths, out, workspace, status, row_start=None):
     _bf16(Q, out)
     P, G, page, D = _pool_sizes(pool, scales)
     shape = Q.shape
@@ -737,6 +737,11 @@ def _pages_attention(Q, pool, scales, tables, lengths, out, workspace, row_start
         checked.append(out)
     if workspace is not None:
         checked.append(workspace)
+    if status is not None:
+        _int32("status words", status)
+        if status.numel() < 1:
+            raise ValueError("the status word is empty")
+        checked.append(status)
     stream = _on_device(*checked)
     if workspace is None:
         workspace = pages_workspace(D, row_start is not None, Q.device)
@@ -752,7 +757,7 @@ def mha_decode_pages(Q, pool, scales, tables, lengths, out=None, *, window=None,
     that receives ``IRON_ERR_TIMEOUT`` when a bounded wait gives up (``pages_status``'s when not given)."""
     if Q.shape[:1] != lengths.shape:
         raise ValueError(f"Q {tuple(Q.shape)} is not one query for each of {tuple(lengths.shape)} requests")
-    P, G, page, D, out, workspace, stream = _pages_attention(Q, pool, scales, tables, lengths, out, workspace)
+    P, G, page, D, out, workspace, stream = _pages_attention(Q, pool, scales, tables, lengths, out, workspace, status)
     call("iron_mha_decode_pages_bf16", Q.data_ptr(), pool.data_ptr(), scales.data_ptr(), P, page, tables.data_ptr(),
          tables.shape[1], lengths.data_ptr(), Q.shape[0], Q.shape[1], G, D, _window(window),
          1.0 / math.sqrt(D) if scale is None else float(scale), workspace.data_ptr(), workspace.numel(),
@@ -772,7 +777,8 @@ def mha_prefill_pages(Q, pool, scales, tables, lengths, row_start, out=None, *, 
         raise ValueError(f"row_start {tuple(row_start.shape)} is not ({B + 1},)")
     if window is not None and not causal:
         raise ValueError("a window goes with the causal mask")
-    P, G, page, D, out, workspace, stream = _pages_attention(Q, pool, scales, tables, lengths, out, workspace, row_start)
+    P, G, page, D, out, workspace, stream = _pages_attention(Q, pool, scales, tables, lengths, out, workspace, status,
+                                                              row_start)
     call("iron_mha_prefill_pages_bf16", Q.data_ptr(), pool.data_ptr(), scales.data_ptr(), P, page, tables.data_ptr(),
          tables.shape[1], lengths.data_ptr(), row_start.data_ptr(), B, Q.shape[0], Q.shape[1], G, D, int(bool(causal)),
          _window(window), 1.0 / math.sqrt(D) if scale is None else float(scale),

@@ -157,3 +157,13 @@ def test_page_step_refuses_tables_whose_tokens_pass_32_bits(page):
 def test_without_a_device_there_is_no_status_word():
     if not torch.cuda.is_available():
         assert _lib.load().iron_mha_pages_status_word() is None
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("status, error", [
+    (torch.zeros(1), TypeError), (torch.zeros(1, dtype=torch.uint8), TypeError), (torch.zeros(0, dtype=I32), ValueError),
+    (torch.zeros(1, dtype=I32), RuntimeError),                       # a word that the device cannot write
+])
+def test_a_status_word_is_one_int32_of_the_device(prompt, status, error):
+    with pytest.raises(error):
+        _attend(prompt, status=status)
