@@ -57,7 +57,9 @@ constexpr float kPtLift = 6.f;        // log2 of what weights are held times
 constexpr float kPtSlack = 8.f;       // log2 of how far the maximum in use may lag
 constexpr int kPtFoldWarps = 8;
 constexpr int kPtSlots = 4;           // items looked up ahead
-constexpr int kPtScales = 4;          // tiles whose scales are held: the converters are two ahead at most
+// Tiles whose scales are held.  Tile n's are written once the last scores of tile n - kStages are done, which the
+// softmax's end with tile n - kStages - 1 precedes: kStages + 1 tiles may be wanted at once.
+constexpr int kPtScales = 4;
 constexpr int kPtPitch = 80;          // bytes between the rows a warp turns its outputs in: 16-byte pieces of 8 rows on 8 bank groups
 constexpr int kPtRoles = 18;          // warps that read them
 
@@ -66,6 +68,7 @@ struct PtCfg {
   static constexpr int kChunks = D / 64;
   static constexpr int kTile = kChunks * kPtSub;
   static constexpr int kStages = D == 128 ? 2 : 3;
+  static_assert(kPtScales >= kStages + 1, "the converters would write over scales that are still read");
   static constexpr int kQ = 0;
   static constexpr int kK = kQ + 2 * kTile;
   static constexpr int kV = kK + kStages * kTile;
