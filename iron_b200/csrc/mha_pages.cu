@@ -447,7 +447,11 @@ mha_pages_kernel(const __grid_constant__ CUtensorMap map, const PagesParams p) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) zero[nt][j] = (m_run[nt][j] == -INFINITY ? 0.f : m_run[nt][j]) - kPgLift;
+          for (int j = 0; j < 2; ++j) {
+            const float m = m_run[nt][j] == -INFINITY ? 0.f : m_run[nt][j], lifted = m - kPgLift;
+            // past 2^27 the difference rounds to a lift of 16, which is past the largest half: none there
+            zero[nt][j] = m - lifted > 15.f ? m : lifted;
+          }
 #pragma unroll
         for (int i = 0; i < U; ++i) {
           const float inv = __shfl_sync(0xffffffffu, inv_v, src0 + i);

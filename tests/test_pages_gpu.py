@@ -733,3 +733,26 @@ def test_status_words(prompt):
         own.fill_(value), word.fill_(value)
         assert torch.equal(call(), call(status=own)) and int(own) == int(word) == value
     word.zero_()
+
+
+# ---------------------------------------------------------------------------- scores of any size
+@pytest.mark.parametrize("H, G, D", [(8, 1, 64), (4, 2, 128), (24, 2, 64)])
+@pytest.mark.parametrize("form", ["decode"])
+def test_one_key_takes_all_at_any_size_of_its_score(form, H, G, D):
+    """A row that sees a single token gives that token's value, be its score 2^-90 or 2^110, of either sign."""
+    from iron_b200 import kernels as K
+
+    B, page = 8, 16
+    lengths = [1] * B if form == "decode" else [2] * B
+    tables, P = R.tables_for(lengths, page, 1)
+    pool, scales = R.cache(P, G, page, D, 3)
+    t, l, first = ints(tables), ints(lengths), torch.arange(0, 2 * B, 2, device="cuda")
+    value = pool[t[:, 0].long(), :, 1, 0].double() * scales[t[:, 0].long(), :, 1].double()[..., None]
+    want = value.repeat_interleave(H // G, 1)
+    for power in range(-100, 101):
+        q = queries(2 * B if form == "prompt" else B, H, D, power + 200) * 2.0 ** power
+        if form == "decode":
+            out = K.mha_decode_pages(q, pool, scales, t, l)
+        else:
+            out = K.mha_prefill_pages(q, pool, scales, t, l, ints(np.arange(B + 1) * 2))[first]
+        assert ((out.double() - want).abs() <= tolerance(want, want.abs())).all(), f"queries times 2^{power}"
