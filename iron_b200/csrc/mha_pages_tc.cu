@@ -55,6 +55,8 @@ constexpr int kPtCostOne = 3, kPtCostTwo = 4, kPtItemCost = 12;
 constexpr int kPtMinShare = 12;
 constexpr float kPtLift = 6.f;        // log2 of what weights are held times
 constexpr float kPtSlack = 8.f;       // log2 of how far the maximum in use may lag
+constexpr float kPtFar = 4194304.f;   // 2^22: scores whose f32 steps reach the size of the lift and the slack
+constexpr float kPtNone = -3.4028235e38f;   // the maximum in use of a row that has none
 constexpr int kPtFoldWarps = 8;
 constexpr int kPtSlots = 4;           // items looked up ahead
 // Tiles whose scales are held.  Tile n's are written once the last scores of tile n - kStages are done, which the
@@ -701,8 +703,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
       const float up = __uint_as_float((uint32_t)(268 - e) << 23);
       me.factor = p.scale_log2 / up;
       // The logarithm of an absent page's scale masks finite scores, but a query that is not finite times the
-      // page's zeros is NaN.  Where a row of this warp has one, no key counts as seen by all (the bound is
-      // kept as its complement), and every step takes the masks below.
+      // page's zeros is NaN.  Where a row of this warp has one, the warp takes the careful way.
       if (__any_sync(0xffffffffu, mx == INFINITY || mx != mx)) it.all_hi = ~it.all_hi;
 #pragma unroll
       for (int k = 0; k < D / 8; ++k) {
@@ -732,9 +733,13 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
     };
     bool have = open_item();
     while (have) {
-      const float factor = me.factor;
+      float factor = it.all_hi < 0 ? 1.f : me.factor;
       const int hi_key = me.hi_key, lo_key = me.lo_key;
-      float m_used = -INFINITY, l = 0.f;
+      float base = kPtNone, l = 0.f;   // the maximum in use less the lift
+      // The careful way, of a warp that has a query that is not finite or a score past kPtFar: no key counts as
+      // seen by all (the bound is kept as its complement), so that every step passes the masks, where
+      // absent pages (an inverse of 0) are masked too and scores are rounded before the maximum is taken
+      // off; a fused product and difference would be off by the score's own rounding, 2^2 and far more.
 
       for (int u = 2 * it.t_lo; u < 2 * it.t_hi && ok; ++u, ++t) {
         const int sub = u & 1, buf = 2 * i + sub;
@@ -750,18 +755,20 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
         uint32_t v[64];
         tmem_ld64_now(col, v);
         // (key scale, log2 of the value scale, its inverse) of each 16 keys
-        const uint4 f[4] = {pt_lds128(sc_at), pt_lds128(sc_at + 16), pt_lds128(sc_at + 32), pt_lds128(sc_at + 48)};
+        uint4 f[4] = {pt_lds128(sc_at), pt_lds128(sc_at + 16), pt_lds128(sc_at + 32), pt_lds128(sc_at + 48)};
         if (key0 < it.all_lo || key0 + 64 > it.all_hi) {
 #pragma unroll
           for (int k = 0; k < 64; ++k)
             if (key0 + k >= hi_key || key0 + k < lo_key) v[k] = 0xff800000u;   // this column does not see the key
-          // absent pages (an inverse of 0), under queries that are not finite; 1.6 % of the eight chunks' time
           if (__builtin_expect(it.all_hi < 0, 0)) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (f[q].z == 0)
+            for (int q = 0; q < 4; ++q) {
+              const float a = score_factor(me.factor, f[q].x);
 #pragma unroll
-                for (int k = 0; k < 16; ++k) v[16 * q + k] = 0xff800000u;
+              for (int k = 0; k < 16; ++k)
+                v[16 * q + k] = f[q].z == 0 ? 0xff800000u : __float_as_uint(fmaf(__uint_as_float(v[16 * q + k]), a, __uint_as_float(f[q].y)));
+              f[q].x = 0x3f800000u; f[q].y = 0;
+            }
           }
         }
         // ---- the maximum ----
@@ -773,10 +780,18 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
           for (int k = 2; k < 16; k += 2) top = max3(top, __uint_as_float(v[16 * q + k]), __uint_as_float(v[16 * q + k + 1]));
           mx = fmaxf(mx, fmaf(top, score_factor(factor, f[q].x), __uint_as_float(f[q].y)));
         }
-        if (__any_sync(0xffffffffu, mx > m_used + kPtSlack)) {
-          const float m_new = fmaxf(m_used, mx);
-          const float corr = m_new == -INFINITY ? 1.f : ex2(m_used - m_new);
-          m_used = m_new;
+        if (__any_sync(0xffffffffu, mx - base > kPtLift + kPtSlack)) {
+          const bool far = fabsf(mx) > kPtFar && mx != -INFINITY;
+          if (it.all_hi >= 0 && __any_sync(0xffffffffu, far)) {   // this step once more: its scores still lie there
+            it.all_hi = ~it.all_hi;
+            factor = 1.f;
+            --u; --t;
+            if (sub) --n_tile;
+            continue;
+          }
+          const float base_new = fmaxf(base, far ? mx : mx - kPtLift);   // a far one takes no lift: it would not come out whole
+          const float corr = ex2(base - base_new);
+          base = base_new;
           l *= corr;
           if (u > 2 * it.t_lo) {
             // once the last step's product is done the outputs lie still: this step's waits for P.
@@ -796,7 +811,6 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
           }
         }
         // ---- weights and their sum: P over the scores' place ----
-        const float base = (m_used == -INFINITY ? 0.f : m_used) - kPtLift;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           uint32_t out[16];
@@ -895,7 +909,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) mha_pages_tc_kernel(const Pages
         }
       }
       if (was.live && !done.whole) {
-        part[kPtRows * D + i * 128 + r] = m_used;
+        part[kPtRows * D + i * 128 + r] = base == kPtNone ? -INFINITY : base;
         part[kPtRows * D + kPtRows + i * 128 + r] = l;
       }
     }

@@ -737,7 +737,7 @@ def test_status_words(prompt):
 
 # ---------------------------------------------------------------------------- scores of any size
 @pytest.mark.parametrize("H, G, D", [(8, 1, 64), (4, 2, 128), (24, 2, 64)])
-@pytest.mark.parametrize("form", ["decode"])
+@pytest.mark.parametrize("form", ["decode", "prompt"])
 def test_one_key_takes_all_at_any_size_of_its_score(form, H, G, D):
     """A row that sees a single token gives that token's value, be its score 2^-90 or 2^110, of either sign."""
     from iron_b200 import kernels as K
@@ -756,3 +756,32 @@ def test_one_key_takes_all_at_any_size_of_its_score(form, H, G, D):
         else:
             out = K.mha_prefill_pages(q, pool, scales, t, l, ints(np.arange(B + 1) * 2))[first]
         assert ((out.double() - want).abs() <= tolerance(want, want.abs())).all(), f"queries times 2^{power}"
+
+
+@pytest.mark.parametrize("form", ["decode", "prompt"])
+@pytest.mark.parametrize("power", [20, 60, -60])
+def test_queries_of_very_large_and_very_small_size(form, power):
+    """Queries times 2^20 and 2^60: one key takes all, and the output is its value to half a bf16 step;
+    times 2^-60: all present keys weigh the same."""
+    from iron_b200 import kernels as K
+
+    n, page, G, H, D = 600, 16, 2, 4, 64
+    tables, P = R.tables_for([n], page, 1)
+    pool, scales = R.cache(P, G, page, D, 3)
+    m = 200 if form == "prompt" else 1
+    q = queries(m, H, D, 1) * 2.0 ** power
+    t, l = ints(tables), ints([n])
+    out = K.mha_prefill_pages(q, pool, scales, t, l, ints([0, m])) if form == "prompt" else K.mha_decode_pages(q, pool, scales, t, l)
+    want, size = R.attention(q, pool, scales, t, [n], [0, m])
+    ids = t[0].long()
+    k = (pool[ids, :, 0].double() * scales[ids, :, 0].double()[..., None, None]).permute(1, 0, 2, 3).reshape(G, -1, D)[:, :n]
+    k = k.repeat_interleave(H // G, 0)
+    s = torch.einsum("rhd,hkd->rhk", q.double(), k) / math.sqrt(D)
+    seen = (torch.arange(n, device="cuda")[None] <= torch.arange(n - m, n, device="cuda")[:, None])[:, None]
+    top = torch.where(seen, s, -math.inf).topk(2, -1).values
+    # f32 products and sums of D terms are off by at most D roundings of the terms' sum (2^-23 each, for sums that
+    # truncate), on either key; e^-40 of weight is far below a half's
+    error = 2 * D * 2.0 ** -23 * (torch.einsum("rhd,hkd->rhk", q.double().abs(), k.abs()).amax(-1) / math.sqrt(D))
+    clear = (top[..., 0] - top[..., 1] > error + 40) if power > 0 else torch.full_like(top[..., 0], True, dtype=torch.bool)
+    assert clear.double().mean() > 0.9
+    check_attention(out[clear], want[clear], size[clear])
