@@ -785,3 +785,158 @@ def test_queries_of_very_large_and_very_small_size(form, power):
     clear = (top[..., 0] - top[..., 1] > error + 40) if power > 0 else torch.full_like(top[..., 0], True, dtype=torch.bool)
     assert clear.double().mean() > 0.9
     check_attention(out[clear], want[clear], size[clear])
+
+
+# ---------------------------------------------------------------------------- writes of more than 1024 rows
+def runs_around_looks(page, rows, seed):
+    """(before, new) of requests whose page runs begin at the last row, the first row and the second row
+    of a look of 32 rows, of one, eight, nine and a page's rows, and then of random lengths, ``rows`` in all."""
+    rng = np.random.default_rng(seed)
+    before, new = [], []
+
+    def bring(n, b=0):
+        before.append(b), new.append(n)
+
+    for n in (1, 8, 9, page, page + 1):
+        for first in (31, 32, 33):
+            while (sum(new) + 1) % 32 != (first + 1) % 32:           # single rows up to the place
+                bring(1, int(rng.integers(0, 3 * page)))
+            bring(n)
+            bring(n, page - 1)
+    while sum(new) < rows:
+        n = int(rng.choice([1, 2, 7, 8, 9, page - 1, page, 3 * page]))
+        bring(min(n, rows - sum(new)), int(rng.integers(0, 2 * page)))
+    return before, new
+
+
+@pytest.mark.parametrize("H, G, D, page, rows", [(4, 2, 64, 16, 1025), (2, 2, 128, 16, 1100), (6, 1, 128, 64, 1503),
+                                                 (2, 1, 64, 256, 3000), (3, 3, 128, 256, 2947), (1, 1, 64, 32, 1056)])
+@pytest.mark.parametrize("kind", ["mixed", "mixed, with infinities and NaN", "rows without slots", "one prompt", "single rows"])
+def test_rope_kv_pages_of_many_rows(H, G, D, page, rows, kind):
+    from iron_b200 import kernels as K
+
+    if kind == "one prompt":
+        before, new = [37], [rows]
+    elif kind == "single rows":
+        before, new = [(5 * i) % (2 * page) for i in range(1100)], [1] * 1100
+    else:
+        before, new = runs_around_looks(page, rows, page + rows)
+    qkv, angles, pool, scales, slots, positions = write_case(H, G, D, page, before, new, page + H, "NaN" in kind)
+    assert len(slots) == sum(new) > 1024
+    if kind == "rows without slots":
+        slots[::97] = -1                                     # holes end a run where they lie in one
+        slots[[31, 32, 63, 64, 65, 96]] = -1
+        # what follows a hole inside a page would share the page with what lies before it: those rows go nowhere
+        for b, n in zip(np.cumsum([0] + new[:-1]), new):
+            hole = False
+            for r in range(b, b + n):
+                hole = (hole or slots[r] < 0) and not (slots[r] >= 0 and slots[r] % page == 0)
+                if hole:
+                    slots[r] = -1
+    with np.errstate(all="ignore"):
+        want = R.write(qkv.float().numpy(), angles.float().numpy(), pool.double().numpy(), scales.numpy(), slots, positions, H, G, D)
+    pool, scales = pool.cuda(), scales.cuda()
+    q = torch.full((len(slots), H, D), 7.0, dtype=BF16, device="cuda")
+    for _ in range(2):                                       # the second finds its own rows and scales there
+        K.rope_kv_pages(qkv.cuda(), angles.cuda(), q, pool, scales, ints(slots), ints(positions), H=H, G=G, D=D)
+        check_write(q, pool, scales, want)
+
+
+# ---------------------------------------------------------------------------- repeats, overlap, mixed steps
+@pytest.mark.parametrize("H, G, D", [(32, 8, 64), (16, 2, 128)])
+@pytest.mark.parametrize("lengths, new", [([2048], [2048]), ([4096] * 16, [7] * 16), ([900, 9001, 3000], [900, 61, 1433]),
+                                          ([300 + 17 * i for i in range(40)], [1] * 38 + [64, 300])])
+def test_the_prompt_form_repeats_itself_bit_for_bit(H, G, D, lengths, new):
+    """Partial results join in a fixed order, whatever the workspace held."""
+    from iron_b200 import kernels as K
+
+    page = 64
+    tables, P = R.tables_for(lengths, page, 1)
+    pool, scales = R.cache(P, G, page, D, 2)
+    start = ints(np.concatenate(([0], np.cumsum(new))))
+    q, t, l = queries(sum(new), H, D, 3), ints(tables), ints(lengths)
+    workspace = K.pages_workspace(D, True)
+    outs = []
+    for fill in (0, 0xFF, 0x3C, 0xFF):
+        outs.append(K.mha_prefill_pages(q, pool, scales, t, l, start, workspace=workspace.fill_(fill)))
+    assert all(torch.equal(outs[0], x) for x in outs[1:])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("singles", [0, 20], ids=["prompts", "prompts and single rows"])
+def test_ragged_calls_on_two_streams_and_in_two_graphs(D, singles):
+    """As for the decode form: calls without a workspace of the caller's own have one each."""
+    from iron_b200 import kernels as K
+
+    H, G, page = 8, 2, 32
+    lengths, new = [9000, 37, 2500, 300] + [100 + i for i in range(singles)], [200, 37, 5, 64] + [1] * singles
+    tables, P = R.tables_for(lengths, page, 1)
+    pool, scales = R.cache(P, G, page, D, 2)
+    start = np.concatenate(([0], np.cumsum(new)))
+    t, l, r = ints(tables), ints(lengths), ints(start)
+    qs = [queries(int(start[-1]), H, D, i) for i in range(4)]
+    want = [R.attention(q, pool, scales, t, lengths, start) for q in qs]
+    K.mha_prefill_pages(qs[0], pool, scales, t, l, r)
+    torch.cuda.synchronize()
+    streams, graphs, outs = [torch.cuda.Stream() for _ in range(4)], [], [torch.empty_like(q) for q in qs]
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            K.mha_prefill_pages(qs[i], pool, scales, t, l, r, outs[i])
+    for _ in range(20):
+        for i in range(4):
+            with torch.cuda.stream(streams[i]):
+                if i < 2:
+                    graphs[i].replay()
+                else:
+                    K.mha_prefill_pages(qs[i], pool, scales, t, l, r, outs[i])
+    torch.cuda.synchronize()
+    for out, w in zip(outs, want):
+        check_attention(out, *w)
+
+
+@pytest.mark.parametrize("B, H, G, D, page, width, P, rows", [(24, 8, 2, 128, 32, 12, 150, 320), (40, 16, 1, 64, 64, 9, 170, 1400),
+                                                             (17, 6, 3, 128, 16, 40, 300, 160)])
+def test_a_mixed_serving_run(B, H, G, D, page, width, P, rows):
+    """More than sixteen requests, most of which bring one row a step and some a prompt's chunk, end, or
+    find no room: every captured step's bookkeeping, cache and outputs against the plain forms."""
+    from iron_b200 import kernels as K
+
+    rng = np.random.default_rng(B)
+    tables, lengths, new = ints(np.full((B, width), -1)), ints(np.zeros(B)), ints(np.zeros(B))
+    pages, ring = ints(rng.permutation(P)), ints([0, P, 0, 0])
+    pool, scales = torch.zeros((P, G, 2, page, D), dtype=F8, device="cuda"), torch.ones((P, G, 2), device="cuda")
+    a = np.arange(width * page)[:, None] * 10000.0 ** (-np.arange(0, D, 2) / D)
+    angles = torch.from_numpy(np.stack((np.cos(a), np.sin(a)), -1).reshape(-1, D)).to(BF16).cuda()
+    qkv = torch.zeros((rows, (H + 2 * G) * D), dtype=BF16, device="cuda")
+    slots, positions, row_start = ints(np.zeros(rows)), ints(np.zeros(rows)), ints(np.zeros(B + 1))
+    q, out = torch.zeros((rows, H, D), dtype=BF16, device="cuda"), torch.zeros((rows, H, D), dtype=BF16, device="cuda")
+
+    def step():
+        K.page_step(tables, lengths, new, pages, ring, page_size=page, rows=rows, lengths_out=lengths, ring_out=ring,
+                    slots=slots, positions=positions, row_start=row_start)
+        K.rope_kv_pages(qkv, angles, q, pool, scales, slots, positions, H=H, G=G, D=D)
+        K.mha_prefill_pages(q, pool, scales, tables, lengths, row_start, out)
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    refused = 0
+    for i in range(16):
+        n = np.where(rng.random(B) < 0.08, -1, np.where(rng.random(B) < (0.5 if i == 0 else 0.1), rng.integers(2, rows // 6, B), 1))
+        new.copy_(ints(n))
+        qkv.copy_(torch.from_numpy(rng.standard_normal(qkv.shape)).to(BF16))
+        before = [x.cpu().numpy() for x in (tables, lengths, pages, ring)]
+        old_pool, old_scales = pool.cpu().double().numpy(), scales.cpu().numpy()
+        graph.replay()
+        torch.cuda.synchronize()
+        step_want = R.page_step(before[0], before[1], n, before[2], before[3], page, rows)
+        check_step((slots, positions, row_start, lengths, ring), tables, pages, step_want)
+        check_write(q, pool, scales, R.write(qkv.cpu().float().numpy(), angles.cpu().float().numpy(), old_pool, old_scales,
+                                             step_want["slots"], step_want["positions"], H, G, D))
+        start = np.minimum(step_want["row_start"], rows)
+        want, size = R.attention(q, pool, scales, tables, step_want["lengths"], start)
+        check_attention(out[: start[-1]], want[: start[-1]], size[: start[-1]])
+        refused += int(step_want["ring"][2])
+    assert (refused > 0) == (B > 17) and int(K.pages_status()) == 0      # the smallest batch finds room for all
