@@ -613,9 +613,9 @@ int iron_decode_step_bf16(const void* const* layer_ptrs, const void* maps, int L
  * the ring holds; it takes its pages from the ring's head.  One that is not served keeps what
  * it had and takes nothing.  Ended requests' pages go to the ring's tail in order, to be taken
  * from the next step on.  Written: the new table entries, the ring's new tail, row_start (B + 1)
- * (every request's rows, served or not), and for each of the `rows` rows slots (page id * page +
- * offset; -1 past the last row, for a request that was not served, and where the page id is not in
- * 0 .. P - 1) and positions;
+ * (every request's rows, served or not: what attention makes of an unserved one's means nothing),
+ * and for each of the `rows` rows slots (page id * page + offset; -1 past the last row, for a
+ * request that was not served, and where the page id is not in 0 .. P - 1) and positions;
  * lengths_out (may be lengths) and ring_out = (head, count, requests not served, rows asked for;
  * may be ring).  At most iron_page_step_max_requests() requests; P * page_size and width * page_size
  * stay below 2^31 (slots and positions are 32-bit). */

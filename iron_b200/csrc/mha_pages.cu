@@ -31,9 +31,9 @@
 //
 // Over ragged rows (row_start) the kernel takes the sequences that bring one row and passes the others.
 //
-// Measured (32 heads over 8): 64 sequences of 2048, heads of 64: 31.9 us (135 MB, 4.2 TB/s, 65 % of a plain
-// copy's rate); one of 120,001, heads of 128: 50.8 us (4.8 TB/s, 74 %); 128 of 3 to 8191, over 4, that hold
-// 141 MB: 36.4 us (3.9 TB/s), 550 MB: 102 us (5.4 TB/s, 83 %); one of 500: 8.9 us.  A long call is bound by
+// Measured (32 heads over 8): 64 sequences of 2048, heads of 64: 32.4 us (135 MB, 4.2 TB/s, 64 % of a plain
+// copy's rate); one of 120,001, heads of 128: 51.1 us (4.8 TB/s, 74 %); 128 of 3 to 8191, over 4, that hold
+// 141 MB: 36.5 us (3.9 TB/s), 550 MB: 102 us (5.4 TB/s, 83 %); one of 500: 9.1 us.  A long call is bound by
 // bytes; in a short one some 13,000 clocks go by before a CTA's first product (share, page ids, scales, copies),
 // and each unit is a chain of conversions, products and exponentials (200 instructions at heads of 64, half
 // of them on the integer pipe).
@@ -810,7 +810,8 @@ extern "C" int iron_mha_prefill_pages_bf16(const void* q, const void* pool, cons
   // 187 and 67 us, 64 x 1 on 3000 185 and 80, 16 x 1 on 300 27.6 and 21.5; where no sequence has one row
   // the decode kernel's launches are lost (8 x 64 rows on 1000: 43.0 and 49.2 us; 64 x 33: 118 and 123).
   // How many there are is known on the device alone, so: where there may be many, and where there
-  // can be nothing else.
+  // can be nothing else.  What the bound costs on either side of it: sixteen requests of one row each wait
+  // 5 us longer than with the split, seventeen that bring more each some 5 us longer than without.
   p.split = B > 16 || rows == 1;
   if (rows > 1)
     if (const int bad = mha_pages_tc(p, D, workspace, (cudaStream_t)stream)) return bad;

@@ -14,7 +14,8 @@
 //   warp 18       walks the share's items and hands them to all through a ring
 // A tile goes in two steps of 64 keys with a buffer of scores each, so that a step's exponentials are
 // taken while the next one's scores are computed.  O stays in tensor memory; it is rescaled only when
-// a row's maximum has grown by more than 2^8 over the one in use, which after the first tiles is seldom.
+// a row's maximum has grown by more than 2^8 over the one in use, which after the first tiles is seldom (the
+// rescaling put off under a bounded slack is a published refinement of the online softmax).
 //
 // What the arithmetic is (scales, halves, weights) is the decode kernel's: Q as halves under a
 // power of two a row, a page's key scale on its scores, the logarithm of its value scale added
@@ -27,8 +28,10 @@
 // launch folds them in order.  Exponentials (16 a clock and SM) and MMAs both need 1024 clocks for
 // 128 columns x 128 keys at D 128.
 //
-// Measured (32 heads over 8): 2048 causal rows, heads of 64: 61 us (282 TFLOP/s); eight chunks of 61 to
-// 1433 rows on 900 to 9001 tokens, heads of 128: 311 us (800 TFLOP/s); 16 x 7 rows on 4096: 74 us.  What
+// Measured (32 heads over 8, a graph of ten calls at 1.965 GHz): 2048 causal rows, heads of 64: 61 us (280
+// TFLOP/s); eight chunks of 61 to 1433 rows on 900 to 9001 tokens, heads of 128: 312 us (795 TFLOP/s), and 345 us
+// (720 TFLOP/s) in a long run of calls, where the power cap holds the clock near 1.78 GHz; 16 x 7 rows on 4096:
+// 73 us.  At its 96 registers a thread the kernel spills 12 (heads of 64) and 32 bytes (128).  What
 // bounds the wide items is the softmax's chain: a step takes 2600 clocks of a half (290 until its scores are
 // there, 560 for the maximum, 1250 for the weights, the rest handing over) where exponentials alone would
 // take 1024, the exponentials' pipe is 41 % busy and the tensor pipe 41 %; registers allow no third

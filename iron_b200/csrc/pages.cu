@@ -25,7 +25,7 @@ namespace iron {
 // rows.  Every CTA of the (one) cluster computes the sums itself: the cluster meets once, after
 // all of its reads of the lengths and the ring's header, so both may be updated in place.
 // Bound by latency: the chain length -> sum -> search -> page id -> slot.  64 requests of a row each:
-// 5.7 us; 509 requests with 16,384 rows: 8.5 us.
+// 5.5 us; 509 requests with 16,384 rows: 8.5 us.
 constexpr int kStepThreads = 1024;
 
 // Inclusive sum over the block of two values at once; `total` gets the block's sums.
@@ -172,10 +172,11 @@ __global__ void __launch_bounds__(kStepThreads) page_step_kernel(
 // Bound by bytes: a row's qkv in, q in bf16 and k, v as codes out.  A page's scale needs the largest
 // magnitude of all of a step's rows of that page before the first code, so the unit of work is a run -- the
 // rows that go to one page -- of one head's keys or values: the CTA that finds its beginning in the slots
-// takes all of it, a thread sixteen elements, in registers between the maximum and the conversion.
+// takes all of it, a thread sixteen elements, held between the maximum and the conversion (at its bound of 64
+// registers the kernel spills 88 bytes, 96 with heads of 128).
 // Every run has one owner, so no atomics and one order.  q is the rest of the grid's.
-// 2048 rows of a prompt, 32 heads over 8 of 128: 10.4 us (47 MB, 4.5 TB/s); 6111 ragged rows, over 4: 29.5 us
-// (121 MB, 4.1 TB/s; issue slots 53 % used: conversions and the angles' table); 64 single rows 4.5 us.
+// 2048 rows of a prompt, 32 heads over 8 of 128: 10.3 us (47 MB, 4.5 TB/s); 6111 ragged rows, over 4: 29.4 us
+// (121 MB, 4.1 TB/s; issue slots 53 % used: conversions and the angles' table); 64 single rows 4.9 us.
 constexpr int kWriteThreads = 256;
 constexpr int kShortRun = 8;       // rows that one warp takes by itself
 constexpr int kHeld = 1;           // 16-element pieces a thread holds in registers: two cost more in occupancy (11.1 us for 10.4)

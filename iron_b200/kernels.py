@@ -617,7 +617,8 @@ def page_step(tables, lengths, new_tokens, pages, ring, *, page_size, rows, leng
 
     Returns ``(slots, positions, row_start, lengths_out, ring_out)``; ``ring_out`` is (head, pages
     free, requests not served, rows asked for).  A request that was not served keeps its length,
-    and its rows' slots are -1, as are those past the last row and those of a page id outside the pool."""
+    and its rows' slots are -1, as are those past the last row and those of a page id outside the pool.
+    ``row_start`` counts a refused request's rows too: what attention returns for them means nothing."""
     if tables.dim() != 2 or lengths.dim() != 1 or new_tokens.shape != lengths.shape or tables.shape[0] != lengths.shape[0]:
         raise ValueError(f"tables {tuple(tables.shape)}, lengths {tuple(lengths.shape)} and new_tokens "
                          f"{tuple(new_tokens.shape)} are not (B, width), (B,) and (B,)")
