@@ -79,7 +79,7 @@ __device__ __forceinline__ int seq_len(const PagesParams& p, int b) {
 }
 __device__ __forceinline__ int seq_rows(const PagesParams& p, int b, int& row0) {
   row0 = min(max(p.row_start[b], 0), p.rows);
-  return max(0, min(p.row_start[b + 1], p.rows) - row0);
+  return max(row0, min(p.row_start[b + 1], p.rows)) - row0;   // no difference that could wrap
 }
 
 // a / b for a >= 0, b > 0: the 64-bit division is a long routine, and seldom needed

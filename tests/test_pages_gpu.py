@@ -940,3 +940,26 @@ def test_a_mixed_serving_run(B, H, G, D, page, width, P, rows):
         check_attention(out[: start[-1]], want[: start[-1]], size[: start[-1]])
         refused += int(step_want["ring"][2])
     assert (refused > 0) == (B > 17) and int(K.pages_status()) == 0      # the smallest batch finds room for all
+
+
+@pytest.mark.parametrize("starts", [[0, 40, -(1 << 31), 60], [30, -(1 << 31), (1 << 31) - 1, -5], [-7, 20, (1 << 31) - 1, -(1 << 31)]])
+@pytest.mark.parametrize("others", [0, 20], ids=["few", "more than sixteen"])
+def test_row_starts_out_of_order_or_out_of_range_stay_inside_the_buffers(starts, others):
+    """Row starts that no step hands out: a request has the rows from its start to the next one, both
+    brought into the buffer, and none where they run backwards."""
+    from iron_b200 import kernels as K
+
+    H, G, D, page, rows = 4, 2, 64, 16, 50
+    lengths = [60, 70, 80] + [5] * others
+    starts = starts + [rows] * others
+    tables, P = R.tables_for(lengths, page, 1)
+    pool, scales = R.cache(P, G, page, D, 2)
+    q, t = queries(rows, H, D, 1), ints(tables)
+    buffer = torch.full((rows + 20, H, D), 9.0, dtype=BF16, device="cuda")
+    out = K.mha_prefill_pages(q, pool, scales, t, ints(lengths), ints(starts), buffer[10:-10])
+    assert (buffer[:10] == 9).all() and (buffer[-10:] == 9).all()
+    mine = [(min(max(a, 0), rows), max(min(max(a, 0), rows), min(max(b, 0), rows))) for a, b in zip(starts, starts[1:])]
+    for b, (r0, r1) in enumerate(mine):
+        if r1 > r0 and not any(c != b and x < r1 and r0 < y for c, (x, y) in enumerate(mine)):    # its rows are no other's too
+            want, size = R.attention(q[r0:r1], pool, scales, t[b:b + 1], lengths[b:b + 1], [0, r1 - r0])
+            check_attention(out[r0:r1], want, size)
